@@ -337,6 +337,48 @@ int spio_layernorm_2d_bwd(void* dx, float* dweight, float* dbias, const void* dy
                           const float* stats, const float* weight, long long rows, int c, void* scratch,
                           size_t scratch_bytes, void* stream);
 
+/* ---- GroupNorm2d ---------------------------------------------------------------------
+ * Group norm over the pixels and c / groups channels of a group of each image, with an affine map
+ * and an activation, on NHWC data; fp32 statistics and sums.  No counterpart in the reference.
+ *   z = (x - mean) * rstd * weight + bias,  y = act(z),  rstd = 1 / sqrt(var + eps)
+ * weight / bias are fp32 [c] or NULL; c is a multiple of 8 and of groups, and c / groups rounded up
+ * to a common multiple with 8 is at most 2048.  n or pixels may be 0.
+ *   fwd: y from x.  stats, if not NULL, receives {mean, rstd} as fp32 [n][groups][2] for the backward
+ *        pass; codes and exponents, if not NULL, the 8-bit form of x (see checkpoint8 below).
+ *   bwd: dx (NULL: not wanted), dweight and dbias (fp32 [c], NULL: not wanted) from dy, stats and
+ *        either x or, if codes and exponents are given, the values they stand for; sums are added in
+ *        a fixed order.  bias is needed where the activation has a slope.
+ * scratch is device memory of at least the given size, 16-byte aligned; its contents do not matter. */
+enum { SPIO_TYPE_F16 = 0, SPIO_TYPE_BF16 = 1, SPIO_TYPE_F32 = 2 };
+enum { SPIO_ACT_NONE = 0, SPIO_ACT_RELU = 1, SPIO_ACT_SILU = 2, SPIO_ACT_GELU = 3 };
+typedef struct spio_groupnorm_2d_desc {
+  long long n, pixels; /* images, pixels (h * w) of an image */
+  int c, groups;
+  int type;       /* SPIO_TYPE_*, of x, y, dy and dx */
+  int activation; /* SPIO_ACT_* */
+  float eps;
+} spio_groupnorm_2d_desc;
+size_t spio_groupnorm_2d_fwd_scratch_bytes(const spio_groupnorm_2d_desc* desc);
+int spio_groupnorm_2d_fwd(void* y, float* stats, void* codes, void* exponents, const void* x, const float* weight,
+                          const float* bias, const spio_groupnorm_2d_desc* desc, void* scratch,
+                          size_t scratch_bytes, void* stream);
+size_t spio_groupnorm_2d_bwd_scratch_bytes(const spio_groupnorm_2d_desc* desc);
+int spio_groupnorm_2d_bwd(void* dx, float* dweight, float* dbias, const void* dy, const void* x, const void* codes,
+                          const void* exponents, const float* stats, const float* weight, const float* bias,
+                          const spio_groupnorm_2d_desc* desc, void* scratch, size_t scratch_bytes, void* stream);
+
+/* ---- 8-bit form of an activation tensor ----------------------------------------------
+ * For activations that are kept for a backward pass: 1.125 bytes a value.  Blocks of 8 consecutive
+ * values (one channel group of a pixel in NHWC order) become 8 signed codes and one exponent byte:
+ * value = code * 2^(exponent - 127).  The scale is the smallest power of two, 2^-126 at least, for
+ * which the block's largest magnitude rounds to at most 127; codes are rounded half to even, and stop
+ * at 63 where the value would leave the range of the tensor's type.  A block that holds an infinity or
+ * a NaN gets the exponent 255 and is restored as NaN.  codes has 8 bytes a block and is 8-byte
+ * aligned, exponents one byte a block, x is 16-byte aligned; blocks may be 0. */
+int spio_checkpoint8_pack(void* codes, void* exponents, const void* x, long long blocks, int type, void* stream);
+int spio_checkpoint8_unpack(void* x, const void* codes, const void* exponents, long long blocks, int type,
+                            void* stream);
+
 /* Number of compiled (r, s, wpg, tpw, pps) variants, and the i-th one. */
 int spio_conv2d_gw8_num_variants(void);
 int spio_conv2d_gw8_variant(int i, int* r, int* s, int* wpg, int* tpw, int* pps);

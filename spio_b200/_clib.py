@@ -51,6 +51,13 @@ class DpExchange(Structure):
                 ("capacity", c_size_t)]
 
 
+class GroupNorm2dDesc(Structure):
+    """struct spio_groupnorm_2d_desc."""
+
+    _fields_ = [("n", c_longlong), ("pixels", c_longlong), ("c", c_int), ("groups", c_int), ("type", c_int),
+                ("activation", c_int), ("eps", c_float)]
+
+
 class BackwardOpts(Structure):
     """struct spio_gw8_backward_opts."""
 
@@ -149,6 +156,14 @@ SIGNATURES = {
     "spio_layernorm_2d_bwd": (
         c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_longlong, c_int,
                 c_void_p, c_size_t, c_void_p]),
+    "spio_groupnorm_2d_fwd_scratch_bytes": (c_size_t, [POINTER(GroupNorm2dDesc)]),
+    "spio_groupnorm_2d_fwd": (
+        c_int, [c_void_p] * 7 + [POINTER(GroupNorm2dDesc), c_void_p, c_size_t, c_void_p]),
+    "spio_groupnorm_2d_bwd_scratch_bytes": (c_size_t, [POINTER(GroupNorm2dDesc)]),
+    "spio_groupnorm_2d_bwd": (
+        c_int, [c_void_p] * 10 + [POINTER(GroupNorm2dDesc), c_void_p, c_size_t, c_void_p]),
+    "spio_checkpoint8_pack": (c_int, [c_void_p, c_void_p, c_void_p, c_longlong, c_int, c_void_p]),
+    "spio_checkpoint8_unpack": (c_int, [c_void_p, c_void_p, c_void_p, c_longlong, c_int, c_void_p]),
     "spio_conv2d_gw8_num_variants": (c_int, []),
     "spio_conv2d_gw8_variant": (
         c_int, [c_int, POINTER(c_int), POINTER(c_int), POINTER(c_int), POINTER(c_int), POINTER(c_int)]),

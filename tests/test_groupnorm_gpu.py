@@ -1,0 +1,293 @@
+"""Group norm with an activation (spio::groupnorm_2d): forward, backward, the 8-bit checkpoint, special values,
+layouts, streams and CUDA graphs, against the definition in float64."""
+
+import itertools
+
+import pytest
+import torch
+from torch import nn
+
+from spio_b200.functional import groupnorm_2d, groupnorm_2d_backward_op, groupnorm_2d_op
+from spio_b200.layers import GroupNorm2d
+from tests.norm_reference import CONST, Reference, assert_within
+
+pytestmark = pytest.mark.gpu
+CL = torch.channels_last
+TYPES = [torch.float16, torch.bfloat16, torch.float32]
+ACTS = ["none", "relu", "silu", "gelu"]
+
+# (n, c, h, w, groups): channels a group from 1 to 2048, groups that straddle pieces of 8 channels (3, 5, 6, 12, 20),
+# one pixel, odd sizes, wide images, more channels than one slab, many images, one image over many CTAs
+SHAPES = [
+    (1, 8, 1, 3, 1), (2, 8, 3, 5, 8), (3, 24, 7, 5, 8), (2, 40, 9, 11, 8), (2, 96, 14, 14, 32), (3, 96, 5, 7, 16),
+    (1, 256, 16, 16, 32), (2, 160, 13, 9, 8), (70, 64, 3, 3, 8), (1, 64, 131, 67, 32), (2, 1024, 4, 4, 1),
+    (1, 2048, 3, 3, 1), (2, 1536, 3, 2, 512), (5, 16, 1, 1, 1), (2, 768, 7, 7, 32), (1, 32, 200, 180, 4),
+    (2, 520, 6, 6, 5), (300, 8, 2, 2, 2),
+]
+
+
+def make(shape, dtype, seed=0, affine=True, offset=0.5):
+    n, c, h, w = shape
+    gen = torch.Generator().manual_seed(seed)
+    x = torch.randn((n, c, h, w), generator=gen) * torch.exp(0.4 * torch.randn(1, c, 1, 1, generator=gen))
+    x = (x + offset * torch.randn(1, c, 1, 1, generator=gen)).to(dtype)
+    dy = torch.randn((n, c, h, w), generator=gen).to(dtype)
+    wt = 1 + 0.3 * torch.randn(c, generator=gen) if affine else None
+    bs = 0.3 * torch.randn(c, generator=gen) if affine else None
+    put = lambda t: None if t is None else (t.cuda().contiguous(memory_format=CL) if t.dim() == 4 else t.cuda())  # noqa: E731
+    return put(x), put(dy), put(wt), put(bs)
+
+
+def check_all(shape, groups, dtype, act, checkpoint8=False, affine=True, seed=0, eps=1e-5, offset=0.5):
+    x, dy, w, b = make(shape, dtype, seed, affine, offset)
+    ref = Reference(x, groups, w, b, eps, act, dy, checkpoint8)
+    leaves = [t.requires_grad_(True) for t in (x, w, b) if t is not None]
+    y = groupnorm_2d(x, groups, w, b, eps, act, checkpoint8)
+    assert y.dtype == dtype and y.is_contiguous(memory_format=CL)
+    assert_within(y, ref.y, ref.y_tol, "y")
+    grads = torch.autograd.grad(y, leaves, dy)
+    assert_within(grads[0], ref.dx, ref.dx_tol, "dx")
+    assert grads[0].dtype == dtype
+    if affine:
+        assert_within(grads[1], ref.dweight, ref.dweight_tol, "dweight")
+        assert_within(grads[2], ref.dbias, ref.dbias_tol, "dbias")
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_forward_and_backward(shape, dtype):
+    act = ACTS[SHAPES.index(shape) % 4]
+    check_all(shape[:4], shape[4], dtype, act, seed=1)
+
+
+@pytest.mark.parametrize("shape", SHAPES[1::2], ids=str)
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_checkpoint8(shape, dtype):
+    act = ACTS[(SHAPES.index(shape) // 2 + 2) % 4]
+    check_all(shape[:4], shape[4], dtype, act, checkpoint8=True, seed=2)
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("checkpoint8", [False, True])
+def test_activations(act, dtype, checkpoint8):
+    check_all((3, 48, 10, 9), 6, dtype, act, checkpoint8, seed=3)
+    check_all((2, 48, 10, 9), 16, dtype, act, checkpoint8, affine=False, seed=4)
+
+
+def test_statistics_of_data_far_from_zero():
+    """An offset of 1000 standard deviations: differences to a pivot keep the variance."""
+    x, _, _, _ = make((2, 64, 40, 30), torch.float32, seed=5)
+    x = (x + 1000).requires_grad_(False)
+    _, stats, _, _ = groupnorm_2d_op(x, None, None, 8, 1e-5, "none", False)
+    ref = Reference(x, 8)
+    torch.testing.assert_close(stats[..., 0].double().cpu(), ref.mean, rtol=2.0 ** -22, atol=0)
+    torch.testing.assert_close(stats[..., 1].double().cpu(), ref.rstd, rtol=2e-5, atol=0)
+    # a constant image has the mean itself and no variance
+    for value in (0.0, 3.0, 1000.0):
+        x = torch.full((2, 24, 37, 21), value, device="cuda").contiguous(memory_format=CL)
+        y, stats, _, _ = groupnorm_2d_op(x, None, None, 8, 1e-5, "none", False)
+        assert torch.equal(y, torch.zeros_like(y)) and bool((stats[..., 0] == value).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("checkpoint8", [False, True])
+def test_nonfinite_values_stay_in_their_group(dtype, bad, checkpoint8):
+    x, dy, w, b = make((3, 32, 9, 8), dtype, seed=6)
+    clean = groupnorm_2d(x, 4, w, b, activation="relu")
+    x[1, 11, 4, 3] = bad                              # group 1 (channels 8 .. 15) of image 1
+    x.requires_grad_(True)
+    y = groupnorm_2d(x, 4, w, b, activation="relu", checkpoint8=checkpoint8)
+    hit = torch.zeros_like(y, dtype=torch.bool)
+    hit[1, 8:16] = True
+    assert bool(y[hit].isnan().all()) and torch.equal(y[~hit], clean[~hit])
+    (dx,) = torch.autograd.grad(y, x, dy)
+    assert bool(dx[hit].isnan().all()) and bool(dx[~hit].isfinite().all())
+
+
+def test_empty_tensors():
+    w, b = torch.ones(16, device="cuda", requires_grad=True), torch.zeros(16, device="cuda", requires_grad=True)
+    for shape, c8 in itertools.product([(0, 16, 4, 4), (3, 16, 0, 5)], [False, True]):
+        x = torch.empty(shape, device="cuda", dtype=torch.float16, requires_grad=True)
+        y = groupnorm_2d(x, 4, w, b, checkpoint8=c8)
+        dx, dw, db = torch.autograd.grad(y, (x, w, b), torch.empty_like(y))
+        assert y.shape == shape and dx.shape == shape
+        assert torch.equal(dw, torch.zeros_like(dw)) and torch.equal(db, torch.zeros_like(db))
+
+
+def test_layouts_offsets_and_expanded_gradients():
+    x, dy, w, b = make((2, 32, 6, 7), torch.float16, seed=7)
+    want = groupnorm_2d(x, 8, w, b, activation="silu")
+    assert torch.equal(groupnorm_2d(x.contiguous(), 8, w, b, activation="silu"), want)       # NCHW order
+    padded = torch.empty(x.numel() + 1, device="cuda", dtype=x.dtype)[1:]                    # off a 16-byte boundary
+    off = padded.view(2, 6, 7, 32).permute(0, 3, 1, 2).copy_(x)
+    assert off.data_ptr() % 16 and torch.equal(groupnorm_2d(off, 8, w, b, activation="silu"), want)
+    wide = torch.randn(2, 64, 6, 7, device="cuda").half().contiguous(memory_format=CL)       # a slice of channels
+    part = wide[:, 16:48]
+    assert torch.equal(groupnorm_2d(part, 8, w, b), groupnorm_2d(part.clone(), 8, w, b))
+    strided = torch.stack([w, w], 1)[:, 0]
+    assert not strided.is_contiguous() and torch.equal(groupnorm_2d(x, 8, strided, b, activation="silu"), want)
+    xs = x.clone().requires_grad_(True)
+    (got,) = torch.autograd.grad(groupnorm_2d(xs, 8, w, b, activation="silu").sum(), xs)     # an expanded scalar
+    (ref,) = torch.autograd.grad(groupnorm_2d(xs, 8, w, b, activation="silu"), xs, torch.ones_like(x))
+    assert torch.equal(got, ref)
+
+
+def test_only_requested_gradients_and_reproducibility():
+    x, dy, w, b = make((4, 64, 28, 28), torch.bfloat16, seed=8)
+    _, stats, _, _ = groupnorm_2d_op(x, w, b, 8, 1e-5, "gelu", False)
+    full = groupnorm_2d_backward_op(dy, x, None, None, stats, w, b, 8, "gelu", True, True, True)
+    again = groupnorm_2d_backward_op(dy, x, None, None, stats, w, b, 8, "gelu", True, True, True)
+    assert all(torch.equal(p, q) for p, q in zip(full, again))
+    for want in itertools.product([False, True], repeat=3):
+        got = groupnorm_2d_backward_op(dy, x, None, None, stats, w, b, 8, "gelu", *want)
+        for g, f, on in zip(got, full, want):
+            assert torch.equal(g, f) if on else g.numel() == 0
+    # a frozen norm: weight and bias without gradients
+    xs = x.clone().requires_grad_(True)
+    (dx,) = torch.autograd.grad(groupnorm_2d(xs, 8, w, b, activation="gelu"), xs, dy)
+    assert torch.equal(dx, full[0])
+
+
+def test_gradient_against_differences():
+    """fp32: the directional derivative of the loss against a central difference in float64 steps of 1e-3 (whose
+    own error is h^2 / 6 of the third derivative, and 2^-23 / h of the outputs' rounding: 1e-3 in all)."""
+    x, dy, w, b = make((2, 16, 5, 6), torch.float32, seed=9)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    for act in ("none", "silu", "gelu"):
+        grads = torch.autograd.grad(groupnorm_2d(x, 4, w, b, activation=act), leaves, dy)
+        for i, leaf in enumerate(leaves):
+            step = torch.randn(leaf.shape, generator=torch.Generator().manual_seed(i)).to(leaf.device)
+            ends = []
+            for sign in (1, -1):
+                moved = [t.detach() + (sign * 1e-3 * step if j == i else 0) for j, t in enumerate(leaves)]
+                ends.append((groupnorm_2d(moved[0], 4, moved[1], moved[2], activation=act).double() * dy.double()).sum())
+            numeric = float(ends[0] - ends[1]) / 2e-3
+            direct = float((grads[i].double() * step.double()).sum())
+            scale = float((grads[i].double() * step.double()).norm()) + float(dy.double().norm())
+            assert abs(numeric - direct) <= 1e-3 * scale, (act, i)
+
+
+def test_autocast_keeps_the_data_type():
+    x, _, w, b = make((2, 32, 6, 6), torch.float32, seed=10)
+    w16 = w.half().requires_grad_(True)
+    with torch.autocast("cuda", dtype=torch.float16):
+        y = groupnorm_2d(x, 4, w16, b, activation="silu")
+        y16 = groupnorm_2d(x.half(), 4, w16, b, activation="silu")
+    assert y.dtype == torch.float32 and y16.dtype == torch.float16
+    assert torch.equal(y, groupnorm_2d(x, 4, w16.float(), b, activation="silu"))
+    y.sum().backward()
+    assert w16.grad.dtype == torch.float16
+
+
+def test_module_takes_the_place_of_torch_layers():
+    torch.manual_seed(0)
+    ref = nn.Sequential(nn.GroupNorm(8, 64), nn.SiLU()).cuda()
+    with torch.no_grad():
+        ref[0].weight.uniform_(0.5, 1.5), ref[0].bias.uniform_(-0.2, 0.2)
+    fused = GroupNorm2d.from_torch_module(ref[0], activation=GroupNorm2d.activation_of(ref[1]))
+    assert fused.weight is ref[0].weight and sorted(fused.state_dict()) == ["bias", "weight"]
+    x = torch.randn(3, 64, 12, 10, device="cuda").contiguous(memory_format=CL).requires_grad_(True)
+    dy = torch.randn_like(x)
+    got, want = fused(x), ref(x)
+    torch.testing.assert_close(got, want, rtol=1e-5, atol=2e-5)
+    params = [x, ref[0].weight, ref[0].bias]
+    for g, r in zip(torch.autograd.grad(got, params, dy), torch.autograd.grad(want, params, dy)):
+        torch.testing.assert_close(g, r, rtol=1e-4, atol=2e-4)
+
+
+def test_streams_and_two_calls_at_once():
+    x, dy, w, b = make((4, 64, 56, 56), torch.float16, seed=11)
+    want = groupnorm_2d(x, 8, w, b, activation="silu")
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    results = []
+    for s in streams:
+        with torch.cuda.stream(s):
+            results += [groupnorm_2d(x, 8, w, b, activation="silu") for _ in range(4)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(r, want) for r in results)
+
+
+@pytest.mark.parametrize("checkpoint8", [False, True])
+def test_captured_training_step(checkpoint8):
+    """Forward and backward captured with a live eager graph of other leaves, replayed on new data, twice in a row;
+    two graphs share nothing."""
+    shape, groups = (4, 96, 14, 14), 32
+    x, dy, w, b = make(shape, torch.float16, seed=12)
+    stays = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    eager = groupnorm_2d(stays[0], groups, stays[1], stays[2], activation="silu")     # kept alive across the capture
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+
+    def step():
+        y = groupnorm_2d(leaves[0], groups, leaves[1], leaves[2], activation="silu", checkpoint8=checkpoint8)
+        return (y.detach(), *torch.autograd.grad(y, leaves, dy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    for _ in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(step())
+    for seed in (13, 14):
+        x2, dy2, w2, b2 = make(shape, torch.float16, seed=seed)
+        with torch.no_grad():
+            for t, v in zip((*leaves, dy), (x2, w2, b2, dy2)):
+                t.copy_(v)
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        want = step()
+        for out in outs:
+            assert all(torch.equal(p, q) for p, q in zip(out, want))
+    torch.autograd.grad(eager, stays, torch.ones_like(eager))
+
+
+def test_refusals():
+    x, _, w, b = make((2, 32, 4, 4), torch.float16)
+    bad = [
+        lambda: groupnorm_2d(x.cpu(), 4),
+        lambda: groupnorm_2d(x.double(), 4),
+        lambda: groupnorm_2d(x[0], 4),
+        lambda: groupnorm_2d(x, 5),
+        lambda: groupnorm_2d(x, 0),
+        lambda: groupnorm_2d(x[:, :12], 4),
+        lambda: groupnorm_2d(x, 4, w.half(), b),
+        lambda: groupnorm_2d(x, 4, w[:16], b),
+        lambda: groupnorm_2d(x, 4, w.cpu(), b),
+        lambda: groupnorm_2d(x, 4, activation="tanh"),
+        lambda: groupnorm_2d(x, 4, eps=-1.0),
+        lambda: groupnorm_2d(torch.zeros(1, 4096, 1, 1, device="cuda"), 1),
+    ]
+    for call in bad:
+        with pytest.raises(Exception):
+            call()
+    torch.cuda.synchronize()
+    with pytest.raises(ValueError):
+        GroupNorm2d(3, 32)
+    with pytest.raises(ValueError):
+        GroupNorm2d(4, 36)
+
+
+def test_offsets_beyond_32_bits():
+    """An fp16 tensor of 4.4 GB: the last image's values are those of the image alone."""
+    n, c, h, w = 70, 64, 700, 700
+    x = torch.empty((n, c, h, w), device="cuda", dtype=torch.float16, memory_format=CL).zero_()
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    x[-1] = torch.randn((c, h, w), device="cuda", generator=gen).half()
+    assert x.numel() > 2 ** 31
+    y, stats, codes, exponents = groupnorm_2d_op(x, None, None, 8, 1e-5, "none", True)
+    one = groupnorm_2d_op(x[-1:].clone(memory_format=CL), None, None, 8, 1e-5, "none", True)
+    # the two sizes may be split over CTAs differently: the statistics agree to their rounding
+    torch.testing.assert_close(stats[-1:], one[1], rtol=CONST, atol=CONST)
+    torch.testing.assert_close(y[-1:], one[0], rtol=2 ** -10, atol=1e-6)
+    assert torch.equal(codes[-1:], one[2]) and torch.equal(exponents[-1:], one[3])
+    assert not bool(y[0].any())
+    dx, dw, db = groupnorm_2d_backward_op(y, None, codes, exponents, stats, None, None, 8, "none", True, True, True)
+    assert bool(dx[-1].isfinite().all()) and not bool(dx[0].any())
+    torch.testing.assert_close(db, y[-1].double().sum((1, 2)).float(), rtol=0, atol=CONST * float(y[-1].double().abs().sum((1, 2)).max()))

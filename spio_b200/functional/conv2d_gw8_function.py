@@ -55,22 +55,8 @@ def _require_cuda(t: torch.Tensor) -> None:
         raise ValueError("spio conv2d_gw8 runs on CUDA devices only (no CPU implementation)")
 
 
-@torch.library.custom_op("spio::conv2d_gw8", mutates_args=())
-def conv2d_gw8(
-    inputs: torch.Tensor,
-    weight: torch.Tensor,
-    bias: Optional[torch.Tensor] = None,
-    stride: int = 1,
-    padding_y: int = 0,
-    padding_x: int = 0,
-    dilation: int = 1,
-    groups: int = 1,
-) -> torch.Tensor:
-    """2-D convolution with group width 8: fp16 channels_last tensors, fp32 accumulation.
-
-    inputs (N, C, H, W) fp16; weight (C, 8, R, S) fp16; bias (C,) fp32 or None; stride and
-    dilation must be 1; groups must equal C // 8.  Returns (N, C, P, Q) fp16 channels_last.
-    """
+def forward_kernels(inputs, weight, bias, stride, padding_y, padding_x, dilation, groups) -> torch.Tensor:
+    """The forward pass without torch's dispatcher."""
     assert inputs.dtype == torch.float16
     assert weight.dtype == torch.float16
     assert bias is None or bias.dtype == torch.float32
@@ -87,6 +73,25 @@ def conv2d_gw8(
     return output
 
 
+@torch.library.custom_op("spio::conv2d_gw8", mutates_args=())
+def conv2d_gw8(
+    inputs: torch.Tensor,
+    weight: torch.Tensor,
+    bias: Optional[torch.Tensor] = None,
+    stride: int = 1,
+    padding_y: int = 0,
+    padding_x: int = 0,
+    dilation: int = 1,
+    groups: int = 1,
+) -> torch.Tensor:
+    """2-D convolution with group width 8: fp16 channels_last tensors, fp32 accumulation.
+
+    inputs (N, C, H, W) fp16; weight (C, 8, R, S) fp16; bias (C,) fp32 or None; stride and
+    dilation must be 1; groups must equal C // 8.  Returns (N, C, P, Q) fp16 channels_last.
+    """
+    return forward_kernels(inputs, weight, bias, stride, padding_y, padding_x, dilation, groups)
+
+
 @conv2d_gw8.register_fake
 def _conv2d_gw8_fake(inputs, weight, bias=None, stride: int = 1, padding_y: int = 0,
                      padding_x: int = 0, dilation: int = 1, groups: int = 1):
@@ -97,21 +102,12 @@ def _conv2d_gw8_fake(inputs, weight, bias=None, stride: int = 1, padding_y: int 
     return inputs.new_empty(params.output_shape).to(memory_format=torch.channels_last)
 
 
-@torch.library.custom_op("spio::conv2d_gw8_backward", mutates_args=())
-def conv2d_gw8_backward_op(
-    inputs: torch.Tensor,
-    weight: torch.Tensor,
-    bias: Optional[torch.Tensor],
-    grad_output: torch.Tensor,
-    padding_y: int,
-    padding_x: int,
-    needs_input_grad: bool,
-    needs_weight_grad: bool,
-    needs_bias_grad: bool,
-) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """(grad_input fp16, grad_weight fp32, grad_bias fp32).  A gradient that was not asked
-    for comes back as an empty (0-element) tensor, because an operator schema cannot return
-    None; :func:`conv2d_gw8_backward` turns those into None for autograd."""
+def backward_kernels(inputs, weight, bias, grad_output, padding_y, padding_x, needs_input_grad, needs_weight_grad,
+                     needs_bias_grad, own_scratch: bool = False,
+                     grad_weight_dtype=None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The backward pass without torch's dispatcher.  ``own_scratch``: the weight gradient's scratch is
+    allocated for this call instead of shared by the calls of a stream; ``grad_weight_dtype``: float32 or
+    float16 instead of the setting of :func:`set_grad_weight_dtype`."""
     assert grad_output.dtype == torch.float16
     assert inputs.dtype == torch.float16
     assert weight.dtype == torch.float16
@@ -123,8 +119,8 @@ def conv2d_gw8_backward_op(
     wgrad_kernel = dgrad_kernel = None
     if needs_weight_grad:
         # The kernel overwrites grad_weight, so no zero fill is needed.
-        grad_weight = torch.empty(params.weight_shape, device=inputs.device, dtype=_grad_weight_dtype,
-                                  memory_format=torch.channels_last)
+        grad_weight = torch.empty(params.weight_shape, device=inputs.device,
+                                  dtype=grad_weight_dtype or _grad_weight_dtype, memory_format=torch.channels_last)
         wgrad_kernel = conv2d_gw8_wgrad_kernel_factory.get_kernel(params, inputs.device)
     grad_input = _absent(inputs, torch.float16)
     if needs_input_grad:
@@ -142,7 +138,7 @@ def conv2d_gw8_backward_op(
     if needs_weight_grad:
         # one call: the input-gradient kernel starts on SMs as the weight-gradient kernels free them
         launch_backward(wgrad_kernel, dgrad_kernel, grad_input, grad_weight, inputs, grad_output, weight,
-                        grad_bias if fused_bias else None)
+                        grad_bias if fused_bias else None, own_scratch=own_scratch)
     elif needs_input_grad:
         dgrad_kernel(grad_input, grad_output, weight, None)
     if _CHECK_STATUS:
@@ -150,6 +146,25 @@ def conv2d_gw8_backward_op(
 
         check_status()
     return grad_input, grad_weight, grad_bias
+
+
+@torch.library.custom_op("spio::conv2d_gw8_backward", mutates_args=())
+def conv2d_gw8_backward_op(
+    inputs: torch.Tensor,
+    weight: torch.Tensor,
+    bias: Optional[torch.Tensor],
+    grad_output: torch.Tensor,
+    padding_y: int,
+    padding_x: int,
+    needs_input_grad: bool,
+    needs_weight_grad: bool,
+    needs_bias_grad: bool,
+) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(grad_input fp16, grad_weight fp32, grad_bias fp32).  A gradient that was not asked
+    for comes back as an empty (0-element) tensor, because an operator schema cannot return
+    None; :func:`conv2d_gw8_backward` turns those into None for autograd."""
+    return backward_kernels(inputs, weight, bias, grad_output, padding_y, padding_x, needs_input_grad,
+                            needs_weight_grad, needs_bias_grad)
 
 
 @conv2d_gw8_backward_op.register_fake

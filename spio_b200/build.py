@@ -48,8 +48,10 @@ def _sources():
     units.append((CSRC / "jit_driver.cpp", OBJ_DIR / "jit_driver.o", []))
     units.append((CSRC / "layernorm_2d.cu", OBJ_DIR / "layernorm_2d.o", []))
     units.append((CSRC / "dp_exchange.cu", OBJ_DIR / "dp_exchange.o", []))
-    for i, name in enumerate(("f16", "bf16", "f32")):
-        units.append((CSRC / "groupnorm_2d_inst.cu", OBJ_DIR / f"groupnorm_2d_{name}.o", [f"-DGN_TYPE={i}"]))
+    for data_type in range(3):
+        for threads in (128, 256):
+            units.append((CSRC / "groupnorm_2d_inst.cu", OBJ_DIR / f"groupnorm_2d_{data_type}_{threads}.o",
+                          [f"-DGN_TYPE={data_type}", f"-DGN_THREADS={threads}"]))
     units.append((CSRC / "groupnorm_2d.cu", OBJ_DIR / "groupnorm_2d.o", []))
     units.append((CSRC / "checkpoint8.cu", OBJ_DIR / "checkpoint8.o", []))
     return units

@@ -36,9 +36,7 @@ checkpoint8_pack_kernel(uint2* __restrict__ codes, unsigned char* __restrict__ e
   for (int k = 0; k < kPieces; ++k) {
     const long long b = first + k * kThreads;
     if (b < blocks) {
-      float f[8];
-      to_floats(v[k], f);
-      const Block8 e = encode_block<T>(f);
+      const Block8 e = encode_block(v[k], values_of(v[k]));
       __stcs(codes + b, e.codes);
       exponents[b] = (unsigned char)e.exponent;
     }
@@ -65,10 +63,8 @@ checkpoint8_unpack_kernel(T* __restrict__ x, const uint2* __restrict__ codes,
   for (int k = 0; k < kPieces; ++k) {
     const long long b = first + k * kThreads;
     if (b < blocks) {
-      float f[8];
-      decode_block(v[k], f);
       Piece<T> o;
-      from_floats(o, f);
+      to_piece(o, decode_block(v[k]));
 #pragma unroll
       for (int i = 0; i < Piece<T>::W; ++i) reinterpret_cast<uint4*>(x + b * 8)[i] = o.u[i];  // read next: keep in L2
     }

@@ -6,8 +6,9 @@ namespace spio_b200 {
 
 enum { kActNone = 0, kActRelu = 1, kActSilu = 2, kActGelu = 3, kActs = 4 };
 
-constexpr int kGnThreads = 256;
-constexpr int kGnMaxSlabPieces = 256;  // a thread owns at most one piece of a pixel's slab
+// Threads of a CTA: the one-launch kernels are built with both, the wide one serves the two-kernel forms and groups
+// that span more pieces of 8 channels than the narrow one has threads.
+constexpr int kGnNarrow = 128, kGnWide = 256;
 
 // An image is cut into slabs of whole groups of channels (sp pieces of 8 channels each, the last
 // one narrower) and its pixels into parts; a CTA works on one part of one slab of one image.
@@ -17,9 +18,20 @@ struct GnGeom {
   int c, pieces;  // channels, c / 8
   int groups, cpg;
   int sp, slabs;        // pieces of a slab, slabs of an image
-  int parts, part_px;   // parts of an image, pixels of each (the last one has fewer)
+  int parts, part_px, part_rest;  // parts of an image; pixels of each, one more in the first part_rest
   float inv_m;          // 1 / (pixels * cpg)
   float eps;
+  unsigned cpg_magic;     // ceil(2^32 / cpg)
+  float inv_sp, inv_pixels;
+  // reductions.  fold: a piece lies within one group; lanes: log2 of the lanes that share a group, of which each takes
+  // every 2^lanes-th value of the rows' runs of `run` values: run_rows rows and run_rest values on; column_lanes:
+  // log2 of the lanes that share a channel
+  int fold, lanes, run, run_rows, run_rest, column_lanes;
+  float inv_run;
+  int slab_groups;  // of a full slab
+  int group_at;     // where the groups' values start in the dynamic shared memory
+  // one launch: log2(parts), slots of a thread's ring and of a quarter of it, quarters of a part, where the ring is
+  int log_parts, slots, batch, batches, data_at;
 };
 
 struct GnKernels {
@@ -27,10 +39,16 @@ struct GnKernels {
   const void* apply[kActs][2];      // [activation][writes codes]
   const void* bwd_sums[kActs][2];   // [activation][reads codes]
   const void* bwd_apply[kActs][2];
+  const void* fwd[kActs][2];        // one launch
+  const void* bwd[kActs][2];
 };
 
-const GnKernels* groupnorm_2d_kernels_f16();
-const GnKernels* groupnorm_2d_kernels_bf16();
-const GnKernels* groupnorm_2d_kernels_f32();
+// type: 0 fp16, 1 bf16, 2 fp32; the narrow tables have the one-launch kernels alone
+const GnKernels* groupnorm_2d_wide_kernels_0();
+const GnKernels* groupnorm_2d_wide_kernels_1();
+const GnKernels* groupnorm_2d_wide_kernels_2();
+const GnKernels* groupnorm_2d_narrow_kernels_0();
+const GnKernels* groupnorm_2d_narrow_kernels_1();
+const GnKernels* groupnorm_2d_narrow_kernels_2();
 
 }  // namespace spio_b200

@@ -5,6 +5,11 @@ Error model.  Half a step of the output's type, plus CONST * 2^-24 times the mag
 sums are taken over at most a few hundred terms a thread and then pairwise, so their relative error stays
 within some tens of 2^-24 of the sum of magnitudes, and an element-wise formula rounds about ten times; the
 16-bit types' activations add 1.5e-7 (2.5 * 2^-24) times their argument.  CONST = 64 covers both.
+
+The mean enters with mean |x| of its group and not with |mean|: a sum of n values in fp32 rounds partial sums of
+up to sum |x|, so its error is of the order 2^-24 * mean |x| after the division by n, in any order of summation, while
+|mean| may be as small as the values happen to cancel.  (Six pixels of three channels with values around 1 and a
+mean of 0.02: four roundings of partial sums near 1 are 4 * 2^-24 = 2.4e-7, above 64 * 2^-24 * 0.045 = 1.7e-7.)
 """
 
 import torch
@@ -76,7 +81,8 @@ class Reference:
         mean, rstd = wide(self.mean), wide(self.rstd)
         z = (v - mean) * rstd * wt + bs
         # rounding of x - mean, of the products and of the statistics
-        z_mag = (v.abs() + mean.abs()) * rstd * wt.abs() + bs.abs()
+        size = wide(grouped.abs().mean(2))                     # mean |x| of the group
+        z_mag = (v.abs() + size) * rstd * wt.abs() + bs.abs()
         self.y = _act(z, act)
         self.y_tol = half_step(self.y, dtype) + CONST * z_mag
         if dy is None:
@@ -84,9 +90,9 @@ class Reference:
         if checkpoint8:
             v = restored(x)
             z = (v - mean) * rstd * wt + bs
-            z_mag = (v.abs() + mean.abs()) * rstd * wt.abs() + bs.abs()
+            z_mag = (v.abs() + size) * rstd * wt.abs() + bs.abs()
         g0 = dy.detach().double().cpu()
-        hat, hat_mag = (v - mean) * rstd, (v.abs() + mean.abs()) * rstd
+        hat, hat_mag = (v - mean) * rstd, (v.abs() + size) * rstd
         g = g0 * _slope(z, act)
         # the slopes' own slope is at most 1.2; ReLU's jumps, so a value next to zero may go either way
         g_tol = g0.abs() * CONST * (1 + 1.2 * z_mag * (act != "none") * (act != "relu"))

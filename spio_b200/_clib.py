@@ -14,6 +14,8 @@ from typing import Optional
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libspio_b200.so"
 
+TORCH_LIB_PATH = LIB_PATH.with_name("libspio_b200_torch.so")
+
 FPROP, DGRAD, WGRAD = 0, 1, 2
 
 
@@ -196,6 +198,24 @@ def load() -> ctypes.CDLL:
         fn.argtypes = argtypes
     _lib = lib
     return lib
+
+
+_torch_ops_loaded = False
+
+
+def load_torch_ops() -> None:
+    """Load the library with the operators that are implemented in C++ (csrc/torch_ops.cpp) once."""
+    global _torch_ops_loaded
+    if _torch_ops_loaded:
+        return
+    import torch
+
+    for path in (LIB_PATH, TORCH_LIB_PATH):
+        if not path.exists():
+            raise RuntimeError(f"{path} is missing: build it with `python -m spio_b200.build` "
+                               "(there is no fallback implementation)")
+    torch.ops.load_library(str(TORCH_LIB_PATH))
+    _torch_ops_loaded = True
 
 
 def last_error() -> str:

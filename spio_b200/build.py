@@ -1,4 +1,5 @@
-"""Build libspio_b200.so (the C-ABI library with the sm_100a kernels) in-tree with nvcc.
+"""Build libspio_b200.so (the C-ABI library with the sm_100a kernels) in-tree with nvcc, and
+libspio_b200_torch.so (PyTorch operators on top of it, see csrc/torch_ops.cpp) with the host compiler.
 
 Run as ``python -m spio_b200.build`` or call :func:`build`.  nvcc cross-compiles for
 sm_100a, so no GPU is needed to build.  Plays the role of the reference's Cython build
@@ -19,6 +20,8 @@ CSRC = PKG_DIR / "csrc"
 LIB_DIR = PKG_DIR / "lib"
 OBJ_DIR = PKG_DIR / "lib" / "obj"
 LIB_PATH = LIB_DIR / "libspio_b200.so"
+TORCH_LIB_PATH = LIB_DIR / "libspio_b200_torch.so"
+TORCH_SOURCE = CSRC / "torch_ops.cpp"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON_FLAGS = ["-std=c++17", "-O3", "-lineinfo", "-Xcompiler", "-fPIC", "-diag-suppress", "177"]
@@ -59,13 +62,19 @@ def _sources():
 
 def _newest_input() -> float:
     deps = list(CSRC.glob("*.cu")) + list(CSRC.glob("*.cuh")) + list(CSRC.glob("*.h"))
-    deps += list(CSRC.glob("*.cpp")) + [PKG_DIR.parent / "include" / "spio_b200.h"]
+    deps += [p for p in CSRC.glob("*.cpp") if p != TORCH_SOURCE] + [PKG_DIR.parent / "include" / "spio_b200.h"]
     return max(p.stat().st_mtime for p in deps if p.exists())
 
 
 def is_current() -> bool:
     """True when the library exists and is newer than every source."""
     return LIB_PATH.exists() and LIB_PATH.stat().st_mtime >= _newest_input()
+
+
+def torch_lib_is_current() -> bool:
+    header = PKG_DIR.parent / "include" / "spio_b200.h"
+    newest = max(p.stat().st_mtime for p in (TORCH_SOURCE, header))
+    return TORCH_LIB_PATH.exists() and TORCH_LIB_PATH.stat().st_mtime >= newest
 
 
 def _run(cmd, verbose):
@@ -77,25 +86,43 @@ def _run(cmd, verbose):
     return res.stdout + res.stderr
 
 
+def build_torch_lib(force: bool = False, verbose: bool = False) -> Path:
+    """Compile the operators implemented in C++ against the installed torch; they call libspio_b200, which lies
+    beside them."""
+    if not force and torch_lib_is_current():
+        return TORCH_LIB_PATH
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(find_nvcc()).resolve().parent.parent
+    _run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-w",
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+          f"-I{root / 'include'}", f"-I{root / 'include' / 'torch' / 'csrc' / 'api' / 'include'}",
+          f"-I{cuda / 'include'}", str(TORCH_SOURCE), "-o", str(TORCH_LIB_PATH),
+          f"-L{LIB_DIR}", "-lspio_b200", "-Wl,-rpath,$ORIGIN",
+          f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch"], verbose)
+    return TORCH_LIB_PATH
+
+
 def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) -> Path:
-    """Compile every translation unit (in parallel) and link the shared library."""
-    if not force and is_current():
-        return LIB_PATH
-    nvcc = find_nvcc()
-    OBJ_DIR.mkdir(parents=True, exist_ok=True)
-    flags = ARCH_FLAGS + COMMON_FLAGS + (["-Xptxas", "-v"] if ptxas_info else [])
+    """Compile every translation unit (in parallel) and link the shared libraries; returns the C-ABI library."""
+    if force or not is_current():
+        nvcc = find_nvcc()
+        OBJ_DIR.mkdir(parents=True, exist_ok=True)
+        flags = ARCH_FLAGS + COMMON_FLAGS + (["-Xptxas", "-v"] if ptxas_info else [])
 
-    def compile_one(unit):
-        src, obj, extra = unit
-        return _run([nvcc, *flags, *extra, "-c", str(src), "-o", str(obj)], verbose)
+        def compile_one(unit):
+            src, obj, extra = unit
+            return _run([nvcc, *flags, *extra, "-c", str(src), "-o", str(obj)], verbose)
 
-    units = _sources()
-    with ThreadPoolExecutor(max_workers=min(len(units), os.cpu_count() or 2)) as ex:
-        logs = list(ex.map(compile_one, units))
-    if ptxas_info:
-        print("\n".join(logs))
-    objs = [str(obj) for _, obj, _ in units]
-    _run([nvcc, *ARCH_FLAGS, "-shared", "-o", str(LIB_PATH), *objs, "-ldl"], verbose)
+        units = _sources()
+        with ThreadPoolExecutor(max_workers=min(len(units), os.cpu_count() or 2)) as ex:
+            logs = list(ex.map(compile_one, units))
+        if ptxas_info:
+            print("\n".join(logs))
+        objs = [str(obj) for _, obj, _ in units]
+        _run([nvcc, *ARCH_FLAGS, "-shared", "-o", str(LIB_PATH), *objs, "-ldl"], verbose)
+    build_torch_lib(force, verbose)
     return LIB_PATH
 
 

@@ -55,24 +55,6 @@ def _require_cuda(t: torch.Tensor) -> None:
         raise ValueError("spio conv2d_gw8 runs on CUDA devices only (no CPU implementation)")
 
 
-def forward_kernels(inputs, weight, bias, stride, padding_y, padding_x, dilation, groups) -> torch.Tensor:
-    """The forward pass without torch's dispatcher."""
-    assert inputs.dtype == torch.float16
-    assert weight.dtype == torch.float16
-    assert bias is None or bias.dtype == torch.float32
-    assert _is_unit(stride)
-    assert _is_unit(dilation)
-    assert groups == inputs.shape[1] // 8
-    params = Conv2dGw8Params.from_tensors(inputs, weight, bias, (padding_y, padding_x))
-    _require_cuda(inputs)
-    output = torch.empty(params.output_shape, device=inputs.device, dtype=torch.float16,
-                         memory_format=torch.channels_last)
-    x, w = to_channels_last(inputs, weight)
-    kernel = conv2d_gw8_kernel_factory.get_kernel(params, inputs.device)
-    kernel(output, x, w, bias.contiguous() if bias is not None else None)
-    return output
-
-
 @torch.library.custom_op("spio::conv2d_gw8", mutates_args=())
 def conv2d_gw8(
     inputs: torch.Tensor,
@@ -89,7 +71,20 @@ def conv2d_gw8(
     inputs (N, C, H, W) fp16; weight (C, 8, R, S) fp16; bias (C,) fp32 or None; stride and
     dilation must be 1; groups must equal C // 8.  Returns (N, C, P, Q) fp16 channels_last.
     """
-    return forward_kernels(inputs, weight, bias, stride, padding_y, padding_x, dilation, groups)
+    assert inputs.dtype == torch.float16
+    assert weight.dtype == torch.float16
+    assert bias is None or bias.dtype == torch.float32
+    assert _is_unit(stride)
+    assert _is_unit(dilation)
+    assert groups == inputs.shape[1] // 8
+    params = Conv2dGw8Params.from_tensors(inputs, weight, bias, (padding_y, padding_x))
+    _require_cuda(inputs)
+    output = torch.empty(params.output_shape, device=inputs.device, dtype=torch.float16,
+                         memory_format=torch.channels_last)
+    x, w = to_channels_last(inputs, weight)
+    kernel = conv2d_gw8_kernel_factory.get_kernel(params, inputs.device)
+    kernel(output, x, w, bias.contiguous() if bias is not None else None)
+    return output
 
 
 @conv2d_gw8.register_fake
@@ -100,52 +95,6 @@ def _conv2d_gw8_fake(inputs, weight, bias=None, stride: int = 1, padding_y: int 
     assert groups == inputs.shape[1] // 8
     params = Conv2dGw8Params.from_tensors(inputs, weight, bias, (padding_y, padding_x))
     return inputs.new_empty(params.output_shape).to(memory_format=torch.channels_last)
-
-
-def backward_kernels(inputs, weight, bias, grad_output, padding_y, padding_x, needs_input_grad, needs_weight_grad,
-                     needs_bias_grad, own_scratch: bool = False,
-                     grad_weight_dtype=None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """The backward pass without torch's dispatcher.  ``own_scratch``: the weight gradient's scratch is
-    allocated for this call instead of shared by the calls of a stream; ``grad_weight_dtype``: float32 or
-    float16 instead of the setting of :func:`set_grad_weight_dtype`."""
-    assert grad_output.dtype == torch.float16
-    assert inputs.dtype == torch.float16
-    assert weight.dtype == torch.float16
-    _require_cuda(inputs)
-    grad_output, inputs, weight = to_channels_last(grad_output, inputs, weight)
-    params = Conv2dGw8Params.from_tensors(inputs, weight, bias, padding=(padding_y, padding_x))
-
-    grad_weight = _absent(inputs, torch.float32)
-    wgrad_kernel = dgrad_kernel = None
-    if needs_weight_grad:
-        # The kernel overwrites grad_weight, so no zero fill is needed.
-        grad_weight = torch.empty(params.weight_shape, device=inputs.device,
-                                  dtype=grad_weight_dtype or _grad_weight_dtype, memory_format=torch.channels_last)
-        wgrad_kernel = conv2d_gw8_wgrad_kernel_factory.get_kernel(params, inputs.device)
-    grad_input = _absent(inputs, torch.float16)
-    if needs_input_grad:
-        grad_input = torch.empty_like(inputs)
-        dgrad_kernel = conv2d_gw8_kernel_factory.get_kernel(params, inputs.device, igrad=True)
-
-    # With an odd number of filter taps the weight-gradient kernel sums grad_output over
-    # n, h, w in the unused half of its last MMA; otherwise torch does that reduction.
-    grad_bias = _absent(inputs, torch.float32)
-    fused_bias = needs_bias_grad and needs_weight_grad and (params.r * params.s) % 2 == 1
-    if needs_bias_grad:
-        grad_bias = (torch.empty(params.k, device=inputs.device, dtype=torch.float32) if fused_bias
-                     else grad_output.sum(dim=(0, 2, 3), dtype=torch.float32))
-
-    if needs_weight_grad:
-        # one call: the input-gradient kernel starts on SMs as the weight-gradient kernels free them
-        launch_backward(wgrad_kernel, dgrad_kernel, grad_input, grad_weight, inputs, grad_output, weight,
-                        grad_bias if fused_bias else None, own_scratch=own_scratch)
-    elif needs_input_grad:
-        dgrad_kernel(grad_input, grad_output, weight, None)
-    if _CHECK_STATUS:
-        from .. import check_status
-
-        check_status()
-    return grad_input, grad_weight, grad_bias
 
 
 @torch.library.custom_op("spio::conv2d_gw8_backward", mutates_args=())
@@ -163,8 +112,44 @@ def conv2d_gw8_backward_op(
     """(grad_input fp16, grad_weight fp32, grad_bias fp32).  A gradient that was not asked
     for comes back as an empty (0-element) tensor, because an operator schema cannot return
     None; :func:`conv2d_gw8_backward` turns those into None for autograd."""
-    return backward_kernels(inputs, weight, bias, grad_output, padding_y, padding_x, needs_input_grad,
-                            needs_weight_grad, needs_bias_grad)
+    assert grad_output.dtype == torch.float16
+    assert inputs.dtype == torch.float16
+    assert weight.dtype == torch.float16
+    _require_cuda(inputs)
+    grad_output, inputs, weight = to_channels_last(grad_output, inputs, weight)
+    params = Conv2dGw8Params.from_tensors(inputs, weight, bias, padding=(padding_y, padding_x))
+
+    grad_weight = _absent(inputs, torch.float32)
+    wgrad_kernel = dgrad_kernel = None
+    if needs_weight_grad:
+        # The kernel overwrites grad_weight, so no zero fill is needed.
+        grad_weight = torch.empty(params.weight_shape, device=inputs.device, dtype=_grad_weight_dtype,
+                                  memory_format=torch.channels_last)
+        wgrad_kernel = conv2d_gw8_wgrad_kernel_factory.get_kernel(params, inputs.device)
+    grad_input = _absent(inputs, torch.float16)
+    if needs_input_grad:
+        grad_input = torch.empty_like(inputs)
+        dgrad_kernel = conv2d_gw8_kernel_factory.get_kernel(params, inputs.device, igrad=True)
+
+    # With an odd number of filter taps the weight-gradient kernel sums grad_output over
+    # n, h, w in the unused half of its last MMA; otherwise torch does that reduction.
+    grad_bias = _absent(inputs, torch.float32)
+    fused_bias = needs_bias_grad and needs_weight_grad and (params.r * params.s) % 2 == 1
+    if needs_bias_grad:
+        grad_bias = (torch.empty(params.k, device=inputs.device, dtype=torch.float32) if fused_bias
+                     else grad_output.sum(dim=(0, 2, 3), dtype=torch.float32))
+
+    if needs_weight_grad:
+        # one call: the input-gradient kernel starts on SMs as the weight-gradient kernels free them
+        launch_backward(wgrad_kernel, dgrad_kernel, grad_input, grad_weight, inputs, grad_output, weight,
+                        grad_bias if fused_bias else None)
+    elif needs_input_grad:
+        dgrad_kernel(grad_input, grad_output, weight, None)
+    if _CHECK_STATUS:
+        from .. import check_status
+
+        check_status()
+    return grad_input, grad_weight, grad_bias
 
 
 @conv2d_gw8_backward_op.register_fake

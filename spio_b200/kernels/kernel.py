@@ -143,15 +143,13 @@ class Kernel:
 
 
 def launch_backward(wgrad_kernel: Kernel, dgrad_kernel: Optional[Kernel], grad_input, grad_weight, inputs,
-                    grad_output, weight, grad_bias=None, own_scratch: bool = False) -> None:
+                    grad_output, weight, grad_bias=None) -> None:
     """Weight gradient, optionally the bias gradient (odd number of filter taps only) and,
     with ``dgrad_kernel``, the input gradient of a layer, through the library's combined entry
     point: weight gradient, reduce and input gradient are chained with programmatic dependent
     launch.  Kernels built into the library and kernels compiled just in time mix freely; the
     latter are passed by their function handles.  ``grad_weight`` may be fp32 (the reference's
-    contract) or fp16 (the parameter's own type, rounded once from the fp32 sum).
-    ``own_scratch`` takes the scratch from torch's allocator for this call: two CUDA graphs captured
-    on one stream then share none."""
+    contract) or fp16 (the parameter's own type, rounded once from the fp32 sum)."""
     kernels = [wgrad_kernel] + ([dgrad_kernel] if dgrad_kernel is not None else [])
     for k in kernels:
         if k._lib is None:
@@ -171,8 +169,7 @@ def launch_backward(wgrad_kernel: Kernel, dgrad_kernel: Optional[Kernel], grad_i
             getattr(wgrad_kernel, "dbias_function_handle", None),
             getattr(dgrad_kernel, "function_handle", None) if dgrad_kernel is not None else None)
         with torch.cuda.device(dev):
-            scratch = (torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev) if own_scratch
-                       else scratch_for(dev, stream, nbytes))
+            scratch = scratch_for(dev, stream, nbytes)
             rc = wgrad_kernel._lib.spio_conv2d_gw8_backward_ex(
                 grad_input.data_ptr() if dgrad_kernel is not None else None, grad_weight.data_ptr(),
                 grad_bias.data_ptr() if grad_bias is not None else None, inputs.data_ptr(),

@@ -19,18 +19,24 @@ perf_model_cache = PerformanceModelCache()
 
 
 class KernelCache:
+    # counts changes that may alter what any cache returns for a shape it has returned a kernel for
+    generation = 0
+
     def __init__(self):
         self._cache: Dict[KernelKey, Kernel] = {}
         self._cache_overlay: Dict[KernelKey, Kernel] = {}
 
     def update_overlay(self, overlay: Dict[KernelKey, Kernel]) -> None:
         """While an overlay is set only its kernels are used."""
+        KernelCache.generation += 1
         self._cache_overlay.update(overlay)
 
     def clear_overlay(self) -> None:
+        KernelCache.generation += 1
         self._cache_overlay.clear()
 
     def clear_cache(self) -> None:
+        KernelCache.generation += 1
         self._cache.clear()
 
     @log_kernel_params

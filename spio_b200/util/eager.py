@@ -1,8 +1,7 @@
 """When an operator may be called without torch's dispatcher.
 
-A custom operator costs 20 to 50 us of host time in eager mode (about 200 us with its backward pass), more than
-the kernels of a small tensor.  Plain eager calls therefore go straight to the library (through
-``torch.autograd.Function`` where a gradient is wanted); everything that has to see an operator -- fake tensors,
+A Python operator costs 20 to 50 us of host time in eager mode (about 200 us with its backward pass), more than
+the kernels of a small tensor.  Plain eager calls therefore go through ``torch.autograd.Function``; everything that has to see an operator -- fake tensors,
 tensor subclasses, tracing and compilation, functorch transforms, forward-mode derivatives, dispatch modes such as
 profilers' counters -- still finds the custom operator.
 """
@@ -26,20 +25,3 @@ def plain_eager(*tensors) -> bool:
             and torch._C._functorch.peek_interpreter_stack() is None
             and torch._C._get_tracing_state() is None
             and forward_ad._current_level < 0)
-
-
-def wants_grad(*tensors) -> bool:
-    if not torch.is_grad_enabled():
-        return False
-    for t in tensors:
-        if t is not None and t.requires_grad:
-            return True
-    return False
-
-
-def call_on(index: int, fn, *args):
-    """``fn(*args, stream)`` with device ``index`` current and its current stream last."""
-    if index == torch.cuda.current_device():
-        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    with torch.cuda.device(index):
-        return fn(*args, torch._C._cuda_getCurrentRawStream(index))

@@ -169,6 +169,45 @@ def test_gradient_against_differences():
             assert abs(numeric - direct) <= 1e-3 * scale, (act, i)
 
 
+def test_absent_weight_or_bias():
+    x, dy, w, b = make((2, 32, 6, 5), torch.float32, seed=15)
+    for weight, bias in ((w, None), (None, b)):
+        ref = Reference(x, 4, weight, bias, 1e-5, "silu", dy)
+        given = (weight if weight is not None else bias).clone().requires_grad_(True)
+        xs = x.clone().requires_grad_(True)
+        y = groupnorm_2d(xs, 4, given if weight is not None else None, given if bias is not None else None, activation="silu")
+        assert_within(y, ref.y, ref.y_tol, "y")
+        dx, dv = torch.autograd.grad(y, (xs, given), dy, retain_graph=True)
+        assert_within(dx, ref.dx, ref.dx_tol, "dx")
+        assert_within(dv, ref.dweight if weight is not None else ref.dbias,
+                      ref.dweight_tol if weight is not None else ref.dbias_tol, "vector")
+        (dv2,) = torch.autograd.grad(y, (given,), dy)      # without the input gradient
+        assert torch.equal(dv, dv2)
+
+
+def test_second_derivatives_are_refused():
+    x, dy, w, b = make((2, 16, 4, 4), torch.float32, seed=16)
+    x.requires_grad_(True)
+    y = groupnorm_2d(x, 4, w, b, activation="silu")
+    (dx,) = torch.autograd.grad(y, x, dy, create_graph=True)
+    with pytest.raises(RuntimeError, match="twice"):
+        dx.square().sum().backward()
+
+
+def test_compiled_model_traces_through_the_operator():
+    """torch.compile sees one opaque operator (eager backend: nothing else is compiled)."""
+    x, _, w, b = make((2, 32, 6, 6), torch.float16, seed=17)
+    layer = GroupNorm2d(4, 32, activation="gelu", checkpoint8=True).cuda()
+    with torch.no_grad():
+        layer.weight.copy_(w), layer.bias.copy_(b)
+    compiled = torch.compile(layer, backend="aot_eager", fullgraph=True)
+    xs, xc = x.clone().requires_grad_(True), x.clone().requires_grad_(True)
+    y, yc = layer(xs), compiled(xc)
+    assert torch.equal(y, yc)
+    y.sum().backward(), yc.sum().backward()
+    assert torch.equal(xs.grad, xc.grad)
+
+
 def test_autocast_keeps_the_data_type():
     x, _, w, b = make((2, 32, 6, 6), torch.float32, seed=10)
     w16 = w.half().requires_grad_(True)

@@ -55,7 +55,7 @@ struct Plan {
   unsigned grid;
   bool one_launch;       // of clusters, else two kernels
   int threads;           // of a CTA
-  int smem;              // dynamic shared memory
+  int smem, slots;       // dynamic shared memory, slots of the ring
   long long rows;        // of the backward pass's partial sums
   size_t stats_bytes;    // forward, two kernels: parts' statistics
   size_t channel_bytes;  // backward: parts' sums for the channels
@@ -108,12 +108,22 @@ int check_desc(const spio_groupnorm_2d_desc* d) {
 
 int cdiv(long long a, long long b) { return (int)((a + b - 1) / b); }
 
-void set_parts(GnGeom* g, int parts) {
+void set_parts(GnGeom* g, int parts, int cluster) {  // cluster: a power of two
   g->parts = parts;
-  g->log_parts = 0;
-  while ((2 << g->log_parts) <= parts) ++g->log_parts;
   g->part_px = g->pixels / parts;
   g->part_rest = g->pixels % parts;
+  g->cluster = cluster;
+  g->log_cluster = 0;
+  while ((1 << g->log_cluster) < cluster) ++g->log_cluster;
+}
+
+// As many parts of an image as there are CTAs for each slab in one filling of the device, but four pixels a thread at
+// least; in pairs, which halves what the second launch has to merge.
+void set_many_parts(GnGeom* g, const Device& dev, bool backward) {
+  const long long want = std::max(1ll, (backward ? 2 : 3) * dev.sms / (g->images * g->slabs));
+  const long long cap = g->pixels / (4 * (kGnWide / g->sp));
+  const int parts = (int)std::max(1ll, std::min(want, cap));
+  set_parts(g, parts >= 2 ? parts / 2 * 2 : 1, parts >= 2 ? 2 : 1);
 }
 
 void set_slabs(GnGeom* g, int unit, int most) {  // slabs of at most `most` units, as even as they get
@@ -122,7 +132,7 @@ void set_slabs(GnGeom* g, int unit, int most) {  // slabs of at most `most` unit
   g->slabs = cdiv(g->pieces, g->sp);
 }
 
-// What the reductions of a CTA need: returns the bytes of shared memory.
+// What the reductions of a CTA need: returns the bytes of shared memory of their arrays.
 int set_reduction(GnGeom* g, int threads, bool backward) {
   g->inv_sp = 1.f / (float)g->sp;
   g->slab_groups = g->sp * 8 / g->cpg;
@@ -135,9 +145,8 @@ int set_reduction(GnGeom* g, int threads, bool backward) {
   g->run_rest = (1 << g->lanes) % g->run;
   g->column_lanes = 0;
   while (g->column_lanes < 5 && (g->sp * 16) << (g->column_lanes + 1) <= threads) ++g->column_lanes;
-  const int plane = threads * 8 * 4;
-  g->group_at = backward ? 2 * plane + threads * 8 : g->fold ? threads * 4 : plane;
-  return g->group_at + g->slab_groups * 8;
+  g->plane = g->fold && !backward ? threads : threads * 8;
+  return 2 * g->plane * 4 + (backward ? threads * 8 : 0);
 }
 
 const GnKernels* kernels_of(int type, bool wide) {
@@ -146,26 +155,32 @@ const GnKernels* kernels_of(int type, bool wide) {
   return type == 0 ? groupnorm_2d_narrow_kernels_0() : type == 1 ? groupnorm_2d_narrow_kernels_1() : groupnorm_2d_narrow_kernels_2();
 }
 
-// Rings of 256 bytes a thread, half as much again where that holds all of a thread's pieces; `bytes`: of a slot.
-void set_ring(Plan* p, int bytes, bool backward) {
+// The ring of the kernels (GnBatch): 64 bytes a thread and batch in pieces of x (and dy).
+void set_ring(Plan* p, int type, int bytes, bool backward) {
   GnGeom& g = p->g;
-  const int pieces = std::max(1, cdiv(cdiv(g.pixels, g.parts), p->threads / g.sp));  // of a thread
-  const int slots = 256 / bytes / 4 * 4;
-  g.batch = cdiv(2 * pieces <= 3 * slots ? pieces : slots, 4);
-  g.slots = 4 * g.batch;
-  g.batches = cdiv(pieces, g.batch);
-  g.data_at = (set_reduction(&g, p->threads, backward) + 2 * g.slab_groups * 8 + 15) / 16 * 16;
-  p->smem = g.data_at + g.slots * p->threads * bytes;
+  const int pieces = cdiv(cdiv(g.pixels, g.parts), p->threads / g.sp);  // of a thread
+  const int batch = (backward ? 4 : 8) / (type == 2 ? 4 : 2);
+  g.batches = std::max(1, cdiv(pieces, batch));
+  p->slots = 4 * batch;
+  const int arrays = set_reduction(&g, p->threads, backward), ring = p->slots * p->threads * bytes;
+  const int groups = (3 * g.slab_groups * 8 + 15) / 16 * 16;
+  if (p->one_launch) {
+    g.planes_at = 0, g.group_at = arrays, g.data_at = arrays + groups;
+    p->smem = g.data_at + ring;
+  } else {
+    g.planes_at = g.data_at = groups, g.group_at = 0;
+    p->smem = groups + std::max(arrays, ring);
+  }
 }
 
 // Which launch to make.  The alternatives differ in the width of a slab, the CTAs of a cluster and their threads, or
 // take two launches; none is best for all sizes.  Narrow slabs and large clusters give CTAs enough to fill the
-// device, wide slabs whole DRAM sectors and lines, few CTAs little bookkeeping, two launches any number of
-// CTAs for one image.  cost() estimates a launch in cycles; its constants are fitted to 2500 measured launches
-// of 60 sizes (all types, activations, directions; 0.01 to 51 million values): the choice takes 3 % longer than the
-// best of each size on average, 28 % at worst.
+// device, wide slabs whole DRAM sectors, few CTAs little bookkeeping, two launches any number of CTAs for one
+// image.  The costs are estimates in cycles with constants fitted to 2500 measured launches of 60 sizes (all types,
+// activations and directions; 0.01 to 51 million values): the choice takes 4 % longer than the best of each size on
+// average, 31 % at worst (8 us instead of 11).
 struct Work {
-  double values, piece_cycles, read, written;  // instructions a warp spends on a piece; bytes
+  double values, piece, read, written;  // instructions a warp spends on a piece in both passes; bytes
 };
 
 Work work_of(const spio_groupnorm_2d_desc* d, bool backward, bool coded) {
@@ -174,16 +189,13 @@ Work work_of(const spio_groupnorm_2d_desc* d, bool backward, bool coded) {
   const double size = d->type == 2 ? 4 : 2;
   Work w;
   w.values = (double)d->n * d->pixels * d->c;
-  w.piece_cycles = (backward ? 110 + 85 * act + (coded ? 20 : 0) : 65 + 30 * act + (coded ? 25 : 0)) + (d->type == 2 ? 15 : 0);
+  w.piece = (backward ? 110 + 85 * act + (coded ? 20 : 0) : 72 + 28 * act + (coded ? 25 : 0)) + (d->type == 2 ? 15 : 0);
   w.read = w.values * (backward ? size + (coded ? 1.125 : size) : size);
   w.written = w.values * (size + (coded && !backward ? 1.125 : 0));
   return w;
 }
 
 constexpr double kBytesPerCycle = 3420.;  // 6500 GB/s at 1.9 GHz
-
-// of the slower of two things that overlap in part
-double overlapped(double a, double b, double rest) { return std::max(a, b) + rest * std::min(a, b); }
 
 double cost_of_one_launch(const Plan& p, const Work& w, const Device& dev, bool backward) {
   const GnGeom& g = p.g;
@@ -192,20 +204,22 @@ double cost_of_one_launch(const Plan& p, const Work& w, const Device& dev, bool 
   const int on_sm = std::max(1, std::min((backward ? 512 : 768) / p.threads, 228 * 1024 / (p.smem + 1024)));
   const double of_sm = std::ceil(ctas / dev.sms), rounds = std::ceil(of_sm / on_sm);
   const double warps = std::min(of_sm, (double)on_sm) * p.threads / 32;
-  const double instructions = of_sm * p.threads / 32 * ((backward ? 250 : 910) + pieces * w.piece_cycles);
-  const double compute = instructions / std::min(2.23, .221 * warps);
+  const double instructions = of_sm * p.threads / 32 * ((backward ? 1060 : 640) + pieces * w.piece);
+  const double compute = instructions / std::min(5.75, .248 * warps);
   const double row = g.sp * 8. * (w.written >= 4 * w.values ? 4 : 2);  // bytes of a pixel
-  const double again = std::max(0., 1. - (double)g.slots / pieces) * w.read * .344;  // from L2
-  const double memory = (w.read + w.written + again) / kBytesPerCycle / (row >= 64 ? 1. : row >= 32 ? .76 : .66);
-  const double sync = g.parts > 1 ? 1250 + 375 * g.log_parts : 0;
-  return .9 * (overlapped(compute, memory, .534) + rounds * (360 + sync)) + (backward ? 9340 : 4840);
+  const double again = std::max(0., 1. - (double)p.slots / pieces) * w.read * 1.4;  // from L2
+  const double memory = (w.read + w.written + again) / kBytesPerCycle / (row >= 64 ? 1. : row >= 32 ? .71 : .69);
+  const double sync = g.cluster > 1 ? 840 + 550 * g.log_cluster : 0;
+  // (the CTAs of an SM start together, and load and compute in turn more than at a time)
+  return .83 * std::max(compute, memory) + 1.17 * std::min(compute, memory) +
+         rounds * ((backward ? 710 : 1800) + sync) + (backward ? 7900 : 4700);
 }
 
 double cost_of_two_launches(const Work& w, const Device& dev, bool backward) {
-  const double compute = w.values / 8 / 32 / dev.sms * (w.piece_cycles + (backward ? 15 : 10)) / 2.615;
+  const double compute = w.values / 8 / 32 / dev.sms * (w.piece + 10) / 2.34;
   const double far = std::min(1., std::max(0., (w.read - 4e7) / 8e7));  // share of the second reading that L2 has lost
-  const double memory = (w.read * (1. + .385 + .615 * far) + w.written) / kBytesPerCycle;
-  return overlapped(compute, memory, .442) + (backward ? 18300 : 14600);
+  const double memory = (w.read * (1. + .87 + .13 * far) + w.written) / kBytesPerCycle;
+  return 1.17 * std::max(compute, memory) + .36 * std::min(compute, memory) + (backward ? 20300 : 15400);
 }
 
 int choose_plan(const spio_groupnorm_2d_desc* d, const Device& dev, bool backward, bool coded, Plan* best) {
@@ -230,10 +244,8 @@ int choose_plan(const spio_groupnorm_2d_desc* d, const Device& dev, bool backwar
   p.one_launch = false;
   p.threads = kGnWide;
   set_slabs(&g, unit, std::max(1, 64 / unit));
-  const long long want = std::max(1ll, (backward ? 2 : 3) * dev.sms / (g.images * g.slabs));
-  const long long cap = g.pixels / (4 * (p.threads / g.sp));
-  set_parts(&g, (int)std::max(1ll, std::min(want, cap)));
-  set_ring(&p, bytes, backward);
+  set_many_parts(&g, dev, backward);
+  set_ring(&p, d->type, bytes, backward);
   *best = p;
   double least = cost_of_two_launches(w, dev, backward);
 
@@ -243,11 +255,11 @@ int choose_plan(const spio_groupnorm_2d_desc* d, const Device& dev, bool backwar
     if (g.sp == sp) continue;
     sp = g.sp;
     for (int parts = 1; parts <= 16 && parts <= g.pixels; parts *= 2) {
-      set_parts(&g, parts);
+      set_parts(&g, parts, parts);
       for (const int threads : {kGnNarrow, kGnWide}) {
         if (sp > threads) continue;
         p.threads = threads;
-        set_ring(&p, bytes, backward);
+        set_ring(&p, d->type, bytes, backward);
         if (p.smem > dev.smem) continue;
         const double cost = cost_of_one_launch(p, w, dev, backward);
         if (cost < least) least = cost, *best = p;
@@ -257,9 +269,10 @@ int choose_plan(const spio_groupnorm_2d_desc* d, const Device& dev, bool backwar
   const GnGeom& b = best->g;
   const long long grid = b.images * b.slabs * b.parts;
   if (grid > 0x7fffffffll) return jit_fail("GroupNorm2d: too many images for one launch");
+  if (((long long)b.part_px + 1) * b.pieces > 0xffffffffll) return jit_fail("GroupNorm2d: an image is too large");
   best->grid = (unsigned)grid;
   best->rows = b.images * b.parts;
-  best->stats_bytes = best->one_launch ? 0 : aligned(sizeof(float2) * (size_t)b.images * b.groups * b.parts);
+  best->stats_bytes = best->one_launch ? 0 : aligned(sizeof(float2) * (size_t)b.images * b.groups * (b.parts / b.cluster));
   best->group_bytes = best->stats_bytes;
   best->channel_bytes = aligned(sizeof(float) * 2 * (size_t)best->rows * b.c);
   return 0;
@@ -349,11 +362,11 @@ int spio_groupnorm_2d_fwd(void* y, float* stats, void* codes, void* exponents, c
   const GnKernels* k = kernels_of(desc->type, p.threads == kGnWide);
   if (p.one_launch) {
     void* args[] = {&y, &stats, &codes, &exponents, (void*)&x, (void*)&weight, (void*)&bias, &p.g};
-    return launch(k->fwd[desc->activation][coded], p.grid, p.threads, p.smem, p.g.parts, stream, args);
+    return launch(k->fwd[desc->activation][coded], p.grid, p.threads, p.smem, p.g.cluster, stream, args);
   }
   if (scratch == nullptr || scratch_bytes < p.stats_bytes) return jit_fail("GroupNorm2d scratch buffer is too small");
   void* sargs[] = {&scratch, (void*)&x, &p.g};
-  if (launch(k->stats, p.grid, p.threads, p.smem, 1, stream, sargs)) return 1;
+  if (launch(k->stats, p.grid, p.threads, p.smem, p.g.cluster, stream, sargs)) return 1;
   void* args[] = {&y, &stats, &codes, &exponents, (void*)&x, (void*)&weight, (void*)&bias, &scratch, &p.g};
   return launch(k->apply[desc->activation][coded], p.grid, p.threads, p.smem, 1, stream, args);
 }
@@ -394,12 +407,12 @@ int spio_groupnorm_2d_bwd(void* dx, float* dweight, float* dbias, const void* dy
   if (p.one_launch) {
     void* args[] = {&dx, &part_channel, (void*)&dy, (void*)&x, (void*)&codes, (void*)&exponents,
                     (void*)&stats, (void*)&weight, (void*)&bias, &p.g};
-    if (launch(k->bwd[desc->activation][coded], p.grid, p.threads, p.smem, p.g.parts, stream, args)) return 1;
+    if (launch(k->bwd[desc->activation][coded], p.grid, p.threads, p.smem, p.g.cluster, stream, args)) return 1;
   } else {
     float2* part_group = dx != nullptr ? reinterpret_cast<float2*>(static_cast<char*>(scratch) + p.channel_bytes) : nullptr;
     void* args[] = {&part_channel, &part_group, (void*)&dy, (void*)&x, (void*)&codes, (void*)&exponents,
                     (void*)&stats, (void*)&weight, (void*)&bias, &p.g};
-    if (launch(k->bwd_sums[desc->activation][coded], p.grid, p.threads, p.smem, 1, stream, args)) return 1;
+    if (launch(k->bwd_sums[desc->activation][coded], p.grid, p.threads, p.smem, p.g.cluster, stream, args)) return 1;
     if (dx != nullptr) {
       void* dargs[] = {&dx, &part_group, (void*)&dy, (void*)&x, (void*)&codes, (void*)&exponents,
                        (void*)&stats, (void*)&weight, (void*)&bias, &p.g};

@@ -8,9 +8,9 @@
 // Statistics and sums are fp32.  A thread owns 8 channels (one piece) of the pixels r, r + R, ... of its
 // CTA's part and sums differences to its first pixel: the pivot is one of the n samples, so
 // (pivot - mean)^2 <= M2 and the cancellation in q - s^2 / n costs at most a factor n of the rounding
-// error, whatever the data's offset.  The threads' sums give the CTA's mean of each group, then their
-// squares are moved to that mean and added; CTAs are merged by means and centred squares.  All in a
-// fixed order: results do not vary from run to run.
+// error, whatever the data's offset.  Threads, lanes and CTAs are then merged by their counts, means and
+// centred squares, in a fixed order: results do not vary from run to run, and the mean of equal values is
+// that value.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -118,6 +118,7 @@ struct GnWork {
   int rows;      // rows of threads: pixels worked on at a time
   int r, p;      // this thread's row and piece; r >= rows: none
   int px0, px;   // first pixel of the part, pixels of it
+  int each, rest;  // pixels of a row, one more in the first `rest` rows
   bool on;
 };
 
@@ -160,6 +161,8 @@ __device__ __forceinline__ GnWork gn_work(const GnGeom& g, unsigned block) {
   w.p = threadIdx.x - w.r * w.sp;
   w.px0 = w.part * g.part_px + min(w.part, g.part_rest);
   w.px = gn_part_pixels(g, w.part);
+  w.each = w.px / w.rows;
+  w.rest = w.px - w.each * w.rows;
   w.on = w.r < w.rows;
   return w;
 }
@@ -169,28 +172,29 @@ __device__ __forceinline__ long long gn_first_group(const GnGeom& g, const GnWor
   return w.image * g.groups + (w.first == 0 ? 0 : w.first / g.sp * g.slab_groups);
 }
 
-// index of the first value of piece (pixel, w.p) of the image
-__device__ __forceinline__ long long gn_offset(const GnGeom& g, const GnWork& w, int pixel) {
-  return (w.image * g.pixels + pixel) * g.c + (long long)(w.first + w.p) * 8;
+// Pieces before the part's first pixel of the slab.  Within the part, 32-bit indices of pieces: one instruction for
+// each address.
+__device__ __forceinline__ long long gn_part_start(const GnGeom& g, const GnWork& w) {
+  return (w.image * g.pixels + w.px0) * g.pieces + w.first;
 }
+__device__ __forceinline__ u32 gn_first_piece(const GnGeom& g, const GnWork& w) { return (u32)w.r * g.pieces + w.p; }
+__device__ __forceinline__ u32 gn_step(const GnGeom& g, const GnWork& w) { return (u32)w.rows * g.pieces; }
 
 // ---------------------------------------------------------------- sums over a CTA
 
 // Shared memory of the reductions: two arrays of a value of each channel of each thread, or of each thread
-// where a piece lies within one group (g.fold), and two values for each of the slab's groups.
+// (where a piece lies within one group, g.fold) two values of each thread; two values for each of the slab's groups.
 struct GnReduce {
   float* a;
-  float* b;        // (backward)
+  float* b;
   float2* folded;  // (backward)
   float2* group;
 };
-constexpr int kGnPlane = kGnThreads * 8;
-
 __device__ __forceinline__ GnReduce gn_reduce(void* at, const GnGeom& g) {
   GnReduce s;
-  s.a = reinterpret_cast<float*>(at);
-  s.b = s.a + kGnPlane;
-  s.folded = reinterpret_cast<float2*>(s.b + kGnPlane);
+  s.a = reinterpret_cast<float*>(reinterpret_cast<char*>(at) + g.planes_at);
+  s.b = s.a + g.plane;
+  s.folded = reinterpret_cast<float2*>(s.b + g.plane);
   s.group = reinterpret_cast<float2*>(reinterpret_cast<char*>(at) + g.group_at);
   return s;
 }
@@ -222,14 +226,14 @@ __device__ __forceinline__ void gn_groups(const GnGeom& g, const GnWork& w, Body
   for (int base = 0; base < w.groups; base += step, k += step) body(k, lane, k < w.groups);
 }
 
-// Calls at(index, channel of the group) for this lane's share of the values of group k: every row's run of them.
+// Calls at(index, channel of the group, row) for this lane's share of the values of group k: every row's run of them.
 template <class At>
 __device__ __forceinline__ void gn_run(const GnGeom& g, const GnWork& w, int k, int lane, At at) {
   const int row = g.fold ? w.sp : w.sp * 8;
   int r = divide(lane, g.inv_run), j = lane - r * g.run;
 #pragma unroll 4
   while (r < w.rows) {
-    at(r * row + k * g.run + j, j);
+    at(r * row + k * g.run + j, j, r);
     r += g.run_rows, j += g.run_rest;
     if (j >= g.run) j -= g.run, ++r;
   }
@@ -268,79 +272,73 @@ __device__ __forceinline__ void spread(const Values& v, float (&f)[8]) {
   }
 }
 
-// Values of the first pixel of the part, one of each group, to which first-order sums are taken (any value near
-// the data does: it keeps the mean of far-off data exact).
-template <class T>
-__device__ __forceinline__ void gn_origin(float (&o)[8], const GnGeom& g, const GnWork& w, const T* __restrict__ x) {
-  if (!w.on) return;
-  const T* at = x + (w.image * g.pixels + w.px0) * g.c + w.first * 8;
-  if (g.fold) {
-    o[0] = (float)at[gn_group(g, w.p * 8) * g.cpg];
-#pragma unroll
-    for (int i = 1; i < 8; ++i) o[i] = o[0];
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = (float)at[gn_group(g, w.p * 8 + i) * g.cpg];
+// Count, mean and centred squares of a set of values, and its union with another set.
+struct GnSet {
+  float n, mean, m2;
+  __device__ __forceinline__ void merge(float n_, float mean_, float m2_) {
+    const float d = mean_ - mean, share = __fdividef(n_, fmaxf(n + n_, 1.f));
+    mean = fmaf(d, share, mean);
+    m2 = fmaf(d * share * n, d, m2 + m2_);
+    n += n_;
   }
-}
+  // with the sets of 2^log neighbouring lanes; lane 0 of them has the union
+  __device__ __forceinline__ void merge_lanes(int log) {
+#pragma unroll
+    for (int i = 0; i < 5; ++i)
+      if (i < log)
+        merge(__shfl_xor_sync(0xffffffffu, n, 1 << i), __shfl_xor_sync(0xffffffffu, mean, 1 << i),
+              __shfl_xor_sync(0xffffffffu, m2, 1 << i));
+  }
+};
 
 // {mean, centred squares} of the groups of the slab over the CTA's pixels, to put(group of the slab, value), by
 // all threads.
 template <class Put>
-__device__ __forceinline__ void gn_group_stats(const GnGeom& g, const GnWork& w, const GnSums& t, const float (&origin)[8],
-                                               const GnReduce& red, Put put) {
-  float s[8], q[8], d[8];
-  const float n = (float)t.n, inv_n = t.n > 0 ? __fdividef(1.f, n) : 0.f;
-  const float inv_values = __fdividef(1.f, (float)w.px * (float)g.cpg);  // values of a group in this part
-  spread(t.s, s), spread(t.q, q), spread(t.away, d);
+__device__ __forceinline__ void gn_group_stats(const GnGeom& g, const GnWork& w, const GnSums& t, const GnReduce& red,
+                                               Put put) {
+  if (w.on) {
+    float mean[8], m2[8], s[8], away[8];
+    const float n = (float)t.n, inv_n = t.n > 0 ? __fdividef(1.f, n) : 0.f;
+    spread(t.s, s), spread(t.q, m2), spread(t.away, away);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float m = s[i] * inv_n;
-    q[i] = not_below_zero(q[i] - s[i] * m);  // about this thread's mean of the channel
-    d[i] = (m - d[i]) - origin[i];           // that mean, from the origin
-    s[i] = n * d[i];
-  }
-  if (w.on) {
-    if (g.fold) red.a[threadIdx.x] = sum8(s);
-    else put8(red.a + threadIdx.x * 8, s);
-  }
-  __syncthreads();
-  gn_groups(g, w, [&](int k, int lane, bool live) {
-    float v = 0.f;
-    if (live) gn_run(g, w, k, lane, [&](int at, int) { v += red.a[at]; });
-    v = sum_lanes(v, g.lanes) * inv_values;
-    if (live && lane == 0) red.group[k].x = v;  // mean, from the origin
-  });
-  __syncthreads();
-  if (w.on) {
-    // (the mean itself is written by a thread that knows the origin: that of the group's first channel)
+    for (int i = 0; i < 8; ++i) {
+      const float d = s[i] * inv_n;
+      m2[i] = fmaf(-s[i], d, m2[i]);
+      mean[i] = d - away[i];
+    }
     if (g.fold) {
-      const int k = gn_group(g, w.p * 8);
-      const float mean = red.group[k].x;
+      float d = 0.f, q = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float e = d[i] - mean;
-        q[i] = fmaf(n * e, e, q[i]);
-      }
-      if (w.r == 0 && w.p * 8 == k * g.cpg) red.group[k].y = mean + origin[0];
-      red.a[threadIdx.x] = sum8(q);
+      for (int i = 1; i < 8; ++i) d += mean[i] - mean[0];
+      const float all = fmaf(d, .125f, mean[0]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) q = fmaf(mean[i] - all, mean[i] - all, q);
+      red.a[threadIdx.x] = all;
+      red.b[threadIdx.x] = fmaf(q, n, sum8(m2));
     } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int k = gn_group(g, w.p * 8 + i);
-        const float mean = red.group[k].x, e = d[i] - mean;
-        q[i] = fmaf(n * e, e, q[i]);
-        if (w.r == 0 && w.p * 8 + i == k * g.cpg) red.group[k].y = mean + origin[i];
-      }
-      put8(red.a + threadIdx.x * 8, q);
+      put8(red.a + threadIdx.x * 8, mean);
+      put8(red.b + threadIdx.x * 8, m2);
     }
   }
   __syncthreads();
+  const float scale = g.fold ? 8.f : 1.f;  // channels of a value
   gn_groups(g, w, [&](int k, int lane, bool live) {
-    float v = 0.f;
-    if (live) gn_run(g, w, k, lane, [&](int at, int) { v += red.a[at]; });
-    v = sum_lanes(v, g.lanes);
-    if (live && lane == 0) put(k, make_float2(red.group[k].y, v));
+    // differences to the lane's first value, which is a mean of members: little cancels
+    float n = 0.f, m0 = 0.f, s = 0.f, q = 0.f;
+    if (live) {
+      gn_run(g, w, k, lane, [&](int at, int, int r) {
+        const float mean = red.a[at], count = (float)(w.each + (r < w.rest)) * scale;
+        if (n == 0.f) m0 = mean;
+        const float d = mean - m0;
+        n += count;
+        s = fmaf(count, d, s);
+        q += fmaf(count * d, d, red.b[at]);
+      });
+    }
+    const float d = n > 0.f ? __fdividef(s, n) : 0.f;
+    GnSet set = {n, m0 + d, fmaf(-s, d, q)};
+    set.merge_lanes(g.lanes);
+    if (live && lane == 0) put(k, make_float2(set.mean, set.m2));
   });
 }
 
@@ -489,12 +487,12 @@ __device__ __forceinline__ void gn_back_groups(const GnGeom& g, const GnWork& w,
     float s = 0.f, q = 0.f;
     if (live) {
       if (g.fold) {
-        gn_run(g, w, k, lane, [&](int at, int) {
+        gn_run(g, w, k, lane, [&](int at, int, int) {
           const float2 v = red.folded[at];
           s += v.x, q += v.y;
         });
       } else {
-        gn_run(g, w, k, lane, [&](int at, int ch) {
+        gn_run(g, w, k, lane, [&](int at, int ch, int) {
           const float f = weight != nullptr ? __ldg(weight + w.first * 8 + k * g.cpg + ch) : 1.f;
           s = fmaf(f, red.a[at], s), q = fmaf(f, red.b[at], q);
         });
@@ -528,8 +526,19 @@ __device__ __forceinline__ void gn_back_channels(const GnGeom& g, const GnWork& 
 // ---------------------------------------------------------------- streaming through shared memory
 //
 // A thread streams its pieces through a ring of slots in shared memory that it alone reads and writes, so the
-// copies need no barrier.  The ring is four batches of g.batch slots, each waited for as a whole and
-// refilled once used; dynamic shared memory is [reductions][groups of the slab: own, merged][ring].
+// copies need no barrier.  The ring is four batches, each waited for as a whole and refilled once used; 256
+// bytes a thread in all, so that the CTAs that registers allow on an SM fit beside each other and have 100 KB or more
+// on their way.  Dynamic shared memory is [reductions][groups of the slab: own, merged][ring]; the kernels that do not
+// come back to the ring reduce in it.
+//
+// The kernels are bound by instructions as much as by memory (a smooth activation takes 6 to 11 a value), so the
+// loops keep their share small: batches have a fixed size and whole ones no bounds checks.
+
+template <class T>
+struct GnBatch {  // slots of a quarter of the ring
+  static constexpr int forward = 8 / (int)sizeof(T);
+  static constexpr int backward = 4 / (int)sizeof(T);
+};
 
 __device__ __forceinline__ void copy_async_16(void* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
@@ -547,57 +556,83 @@ __device__ __forceinline__ void copy_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
 }
 
-// A thread's passes over its `count` pieces through the ring: issue(slot, piece) requests a piece, use(slot, piece)
-// works on it.  The ring's first filling:
-template <class Issue>
-__device__ __forceinline__ void gn_request(const GnGeom& g, int count, Issue issue) {
-  const int size = g.batch;
-  for (int k = 0; k < 4 * size; k += size) {
-    for (int i = k; i < min(k + size, count); ++i) issue(i, i);
-    copy_commit();
+// A thread's passes over its `count` pieces through the ring, `step` pieces apart: issue(slot, offset) requests a piece,
+// use(slot, offset) works on it.  The ring's first filling:
+template <int B, class Issue>
+__device__ __forceinline__ void gn_request(int count, u32 first, u32 step, Issue issue) {
+#pragma unroll
+  for (int k = 0; k < 4 * B; ++k) {
+    if (k < count) issue(k, first + k * step);
+    if (k % B == B - 1) copy_commit();
+  }
+}
+
+// issue() for the pieces i, i + 1, ... of a batch
+template <int B, class Issue>
+__device__ __forceinline__ void gn_refill(int slot, int i, int count, u32 offset, u32 step, Issue issue) {
+  if (i + B <= count) {
+#pragma unroll
+    for (int k = 0; k < B; ++k) issue(slot + k, offset + k * step);
+  } else {
+#pragma unroll
+    for (int k = 0; k < B - 1; ++k)
+      if (i + k < count) issue(slot + k, offset + k * step);
+  }
+}
+
+template <int B, class Use>
+__device__ __forceinline__ void gn_use(int slot, int i, int count, u32 offset, u32 step, Use use) {
+  if (i + B <= count) {
+#pragma unroll
+    for (int k = 0; k < B; ++k) use(slot + k, offset + k * step);
+  } else {
+#pragma unroll
+    for (int k = 0; k < B - 1; ++k)
+      if (i + k < count) use(slot + k, offset + k * step);
   }
 }
 
 // Forwards, behind gn_request.
-template <class Issue, class Use>
-__device__ __forceinline__ void gn_forwards(const GnGeom& g, int count, Issue issue, Use use) {
-  const int size = g.batch;
+template <int B, class Issue, class Use>
+__device__ __forceinline__ void gn_forwards(int count, u32 first, u32 step, Issue issue, Use use) {
+  u32 offset = first;
   int slot = 0;
-  for (int k = 0; k < count; k += size) {
+  for (int i = 0; i < count; i += B) {
     copy_wait<3>();
-    const int last = min(k + size, count);
-#pragma unroll 2
-    for (int i = k; i < last; ++i) use(slot + i - k, i);
-    for (int i = k + 4 * size; i < min(k + 5 * size, count); ++i) issue(slot + i - k - 4 * size, i);
+    gn_use<B>(slot, i, count, offset, step, use);
+    gn_refill<B>(slot, i + 4 * B, count, offset + 4 * B * step, step, issue);
     copy_commit();
-    slot = slot == 3 * size ? 0 : slot + size;
+    offset += B * step;
+    slot = (slot + B) & (4 * B - 1);
   }
   copy_wait<0>();
 }
 
-// Backwards, behind gn_forwards: the last four batches are in the ring.
-template <class Issue, class Use>
-__device__ __forceinline__ void gn_backwards(const GnGeom& g, int count, Issue issue, Use use) {
-  const int size = g.batch;
-  // The same number of batches for all threads, although some have fewer pieces: a batch is requested again four
-  // batches ahead of its use, or was among the thread's last four anyway.
-  const int batches = g.batches;
-  int slot = ((batches - 1) & 3) * size;
-  for (int j = batches - 1; j >= 0; --j) {
-    if (j < batches - 4) copy_wait<3>();
-    const int k = j * size, last = min(k + size, count);
-#pragma unroll 2
-    for (int i = k; i < last; ++i) use(slot + i - k, i);
-    if (j >= 4)
-      for (int i = k - 4 * size; i < min(k - 3 * size, count); ++i) issue(slot + i - k + 4 * size, i);
+// Backwards, behind gn_forwards: the last four batches are in the ring.  The same number of batches for all
+// threads, although some have fewer pieces: a batch is requested again four batches ahead of its use, or was
+// among the thread's last four anyway.
+template <int B, class Issue, class Use>
+__device__ __forceinline__ void gn_backwards(int batches, int count, u32 first, u32 step, Issue issue, Use use) {
+  u32 offset = first + (u32)((batches - 1) * B) * step;
+  int slot = ((batches - 1) & 3) * B;
+  for (int i = (batches - 1) * B; i >= 0; i -= B) {
+    if (i < (batches - 4) * B) copy_wait<3>();
+    gn_use<B>(slot, i, count, offset, step, use);
+    if (i >= 4 * B) gn_refill<B>(slot, i - 4 * B, count, offset - 4 * B * step, step, issue);
     copy_commit();
-    slot = slot == 0 ? 3 * size : slot - size;
+    offset -= B * step;
+    slot = (slot - B) & (4 * B - 1);
   }
 }
 
 // Slots of the part that this thread works on.
 __device__ __forceinline__ int gn_count(const GnWork& w) {
-  return w.on && w.r < w.px ? (w.px - w.r + w.rows - 1) / w.rows : 0;
+  return w.on ? w.each + (w.r < w.rest) : 0;
+}
+
+template <class T>
+__device__ __forceinline__ T* piece_at(T* p, u32 at) {
+  return p + (size_t)at * 8;
 }
 
 // A piece kept in shared memory: W words, a plane of the CTA's slots apart.
@@ -617,53 +652,56 @@ __device__ __forceinline__ void keep_piece(uint4* slot, int plane, const T* from
 // The forward pass of a piece: y, and the 8-bit form of the input.
 template <class T, int ACT, bool CODES>
 __device__ __forceinline__ void gn_write(T* __restrict__ y, uint2* __restrict__ codes,
-                                         unsigned char* __restrict__ exponents, long long at, const Piece<T>& v,
+                                         unsigned char* __restrict__ exponents, u32 at, const Piece<T>& v,
                                          const GnChannels& c) {
   const Values f = values_of(v);
   if (CODES) {
     const Block8 b = encode_block(v, f);
-    __stcs(codes + (at >> 3), b.codes);
-    exponents[at >> 3] = (unsigned char)b.exponent;
+    __stcs(codes + at, b.codes);
+    exponents[at] = (unsigned char)b.exponent;
   }
-  store_piece(y + at, gn_forward<T, ACT>(f, c));
+  store_piece(piece_at(y, at), gn_forward<T, ACT>(f, c));
 }
 
 // The norm's input in the ring: pieces of x, or codes (8 bytes a slot) and the 4-byte words that hold their
-// exponents.
+// exponents.  `start`: pieces before the part.
 template <class T, bool CODES>
 struct GnKept {
+  static constexpr int plane = 4 * GnBatch<T>::backward * kGnThreads;
   uint4* slots;
   const T* x;
-  __device__ __forceinline__ GnKept(char* at, int, const T* x_, const uint2*, const unsigned char*, long long)
-      : slots(reinterpret_cast<uint4*>(at) + threadIdx.x), x(x_) {}
-  __device__ __forceinline__ void issue(int slot, int plane, long long at) {
-    keep_piece(slots + slot * kGnThreads, plane, x + at);
-  }
-  __device__ __forceinline__ Values values(int k, int plane, long long) const {
-    return values_of(kept_piece<T>(slots + k * kGnThreads, plane));
+  __device__ __forceinline__ GnKept(char* at, const GnGeom&, long long start, const T* x_, const uint2*, const unsigned char*)
+      : slots(reinterpret_cast<uint4*>(at) + threadIdx.x), x(x_ + start * 8) {}
+  __device__ __forceinline__ void issue(int slot, u32 at) { keep_piece(slots + slot * kGnThreads, plane, piece_at(x, at)); }
+  __device__ __forceinline__ Values values(int slot, u32) const {
+    return values_of(kept_piece<T>(slots + slot * kGnThreads, plane));
   }
 };
 template <class T>
 struct GnKept<T, true> {
+  static constexpr int plane = 4 * GnBatch<T>::backward * kGnThreads;
   uint2* slots;
   u32* words;
   const uint2* codes;
-  const unsigned char* exponents;
-  long long blocks;
-  __device__ __forceinline__ GnKept(char* at, int plane, const T*, const uint2* codes_, const unsigned char* exponents_,
-                                    long long blocks_)
+  const unsigned char* exponents;  // at a word that begins `shift` bytes before the part's
+  u32 shift, bytes;                // bytes: of the exponents from there on (or 2^32 - 1)
+  __device__ __forceinline__ GnKept(char* at, const GnGeom& g, long long start, const T*, const uint2* codes_,
+                                    const unsigned char* exponents_)
       : slots(reinterpret_cast<uint2*>(at) + threadIdx.x),
-        words(reinterpret_cast<u32*>(at + 8 * (size_t)plane) + threadIdx.x),
-        codes(codes_), exponents(exponents_), blocks(blocks_) {}
-  __device__ __forceinline__ void issue(int k, int, long long at) {
-    const long long block = at >> 3, word = block & ~3ll;
-    copy_async_8(slots + k * kGnThreads, codes + block);
-    copy_async_4(words + k * kGnThreads, exponents + word, (int)min(4ll, blocks - word));
+        words(reinterpret_cast<u32*>(at + 8 * plane) + threadIdx.x),
+        codes(codes_ + start),
+        exponents(exponents_ + (start & ~3ll)),
+        shift((u32)start & 3u),
+        bytes((u32)min(g.images * g.pixels * g.pieces - (start & ~3ll), 0xffffffffll)) {}
+  __device__ __forceinline__ void issue(int slot, u32 at) {
+    const u32 word = (at + shift) & ~3u;
+    copy_async_8(slots + slot * kGnThreads, codes + at);
+    copy_async_4(words + slot * kGnThreads, exponents + word, (int)min(4u, bytes - word));
   }
-  __device__ __forceinline__ Values values(int k, int, long long at) const {
+  __device__ __forceinline__ Values values(int slot, u32 at) const {
     Block8 b;
-    b.codes = slots[k * kGnThreads];
-    b.exponent = (words[k * kGnThreads] >> ((int)(at >> 3) & 3) * 8) & 255u;
+    b.codes = slots[slot * kGnThreads];
+    b.exponent = (words[slot * kGnThreads] >> ((at + shift) & 3u) * 8) & 255u;
     return decode_block(b);
   }
 };
@@ -671,193 +709,26 @@ struct GnKept<T, true> {
 // What the backward passes read: dy and the norm's input.
 template <class T, bool CODES>
 struct GnBackRing {
-  int plane;
+  static constexpr int plane = 4 * GnBatch<T>::backward * kGnThreads;
   uint4* grads;
   const T* dy;
   GnKept<T, CODES> kept;
-  __device__ __forceinline__ GnBackRing(uint4* dynamic, const GnGeom& g, const T* dy_, const T* x, const uint2* codes,
-                                        const unsigned char* exponents)
-      : plane(g.slots * kGnThreads),
-        grads(reinterpret_cast<uint4*>(reinterpret_cast<char*>(dynamic) + g.data_at) + threadIdx.x),
-        dy(dy_),
-        kept(reinterpret_cast<char*>(dynamic) + g.data_at + (size_t)g.slots * kGnThreads * 16 * Piece<T>::W,
-             g.slots * kGnThreads, x, codes, exponents, g.images * g.pixels * g.pieces) {}
-  __device__ __forceinline__ void issue(int slot, long long at) {
-    keep_piece(grads + slot * kGnThreads, plane, dy + at);
-    kept.issue(slot, plane, at);
+  __device__ __forceinline__ GnBackRing(uint4* dynamic, const GnGeom& g, long long start, const T* dy_, const T* x,
+                                        const uint2* codes, const unsigned char* exponents)
+      : grads(reinterpret_cast<uint4*>(reinterpret_cast<char*>(dynamic) + g.data_at) + threadIdx.x),
+        dy(dy_ + start * 8),
+        kept(reinterpret_cast<char*>(dynamic) + g.data_at + plane * 16 * Piece<T>::W, g, start, x, codes, exponents) {}
+  __device__ __forceinline__ void issue(int slot, u32 at) {
+    keep_piece(grads + slot * kGnThreads, plane, piece_at(dy, at));
+    kept.issue(slot, at);
   }
-  __device__ __forceinline__ Values input(int slot, long long at) const { return kept.values(slot, plane, at); }
+  __device__ __forceinline__ Values input(int slot, u32 at) const { return kept.values(slot, at); }
   __device__ __forceinline__ Values grad(int slot) const {
     return values_of(kept_piece<T>(grads + slot * kGnThreads, plane));
   }
 };
 
-// ---------------------------------------------------------------- two launches
-//
-// For a few large images: any number of CTAs works on an image, the sums go through memory, and the second launch
-// reads the input again.  It may ask for it before the first has ended (its inputs were there before that began) and
-// goes through the data backwards, so that it finds in L2 what the first launch read last.
-
-// part_stats[(image * groups + group) * parts + part] = {mean, centred squares} over the part's pixels
-template <class T>
-__global__ void __launch_bounds__(kGnThreads, 768 / kGnThreads)
-groupnorm_2d_stats_kernel(float2* __restrict__ part_stats, const T* __restrict__ x, const GnGeom g) {
-  extern __shared__ uint4 dynamic[];
-  const GnReduce red = gn_reduce(dynamic, g);
-  const int plane = g.slots * kGnThreads;
-  uint4* data = reinterpret_cast<uint4*>(reinterpret_cast<char*>(dynamic) + g.data_at) + threadIdx.x;
-  grid_dependency_wait();
-  grid_dependency_launch_dependents();
-  const GnWork w = gn_work(g, blockIdx.x);
-  const int count = gn_count(w);
-  const long long first = gn_offset(g, w, w.px0 + w.r), step = (long long)w.rows * g.c;
-  const auto issue = [&](int slot, int k) { keep_piece(data + slot * kGnThreads, plane, x + first + k * step); };
-  gn_request(g, count, issue);
-  float origin[8];
-  gn_origin(origin, g, w, x);
-  GnSums t;
-  t.clear();
-  if (count > 0) t.start(values_of(load_piece(x + first)));
-  gn_forwards(g, count, issue,
-              [&](int slot, int) { t.add(values_of(kept_piece<T>(data + slot * kGnThreads, plane))); });
-  const long long first_group = gn_first_group(g, w);
-  gn_group_stats(g, w, t, origin, red, [&](int k, float2 v) { part_stats[(first_group + k) * g.parts + w.part] = v; });
-}
-
-// Mean and rstd of the slab's groups from the parts' values, into stat[]; all threads, synchronised.
-__device__ __forceinline__ void gn_merge_parts(float2* stat, const GnGeom& g, const GnWork& w,
-                                               const float2* __restrict__ part_stats) {
-  const long long first_group = gn_first_group(g, w);
-  const int lane = threadIdx.x & 31;
-  for (int k = threadIdx.x >> 5; k < w.groups; k += kGnThreads / 32) {
-    const float2* ps = part_stats + (first_group + k) * g.parts;
-    const float m0 = __ldcg(ps).x;
-    float s = 0.f, q = 0.f;
-    for (int i = lane; i < g.parts; i += 32) {
-      const float n = (float)gn_part_pixels(g, i);
-      s = fmaf(n, __ldcg(ps + i).x - m0, s);
-    }
-    s = fmaf(sum_lanes(s, 5), g.inv_pixels, m0);
-    for (int i = lane; i < g.parts; i += 32) {
-      const float n = (float)gn_part_pixels(g, i) * (float)g.cpg;
-      const float2 v = __ldcg(ps + i);
-      const float d = v.x - s;
-      q += fmaf(n * d, d, v.y);
-    }
-    q = sum_lanes(q, 5);
-    if (lane == 0) stat[k] = make_float2(s, rsqrtf(fmaf(q, g.inv_m, g.eps)));
-  }
-  __syncthreads();
-}
-
-template <class T, int ACT, bool CODES>
-__global__ void __launch_bounds__(kGnThreads, 768 / kGnThreads)
-groupnorm_2d_apply_kernel(T* __restrict__ y, float2* __restrict__ stats, uint2* __restrict__ codes,
-                          unsigned char* __restrict__ exponents, const T* __restrict__ x,
-                          const float* __restrict__ weight, const float* __restrict__ bias,
-                          const float2* __restrict__ part_stats, const GnGeom g) {
-  extern __shared__ uint4 dynamic[];
-  float2* stat = gn_reduce(dynamic, g).group;
-  const int plane = g.slots * kGnThreads;
-  uint4* data = reinterpret_cast<uint4*>(reinterpret_cast<char*>(dynamic) + g.data_at) + threadIdx.x;
-  const GnWork w = gn_work(g, gridDim.x - 1 - blockIdx.x);
-  const int count = gn_count(w);
-  const long long first = gn_offset(g, w, w.px0 + w.r), step = (long long)w.rows * g.c;
-  const auto issue = [&](int slot, int k) { keep_piece(data + slot * kGnThreads, plane, x + first + k * step); };
-  gn_request(g, count, issue);
-  grid_dependency_wait();
-  grid_dependency_launch_dependents();
-  gn_merge_parts(stat, g, w, part_stats);
-  if (stats != nullptr && w.part == 0) {
-    for (int k = threadIdx.x; k < w.groups; k += kGnThreads) stats[gn_first_group(g, w) + k] = stat[k];
-  }
-  if (!w.on) return;
-  GnChannels c;
-  gn_channels(c, g, w, gn_affine(w, weight, bias), [&](int k) { return stat[k]; });
-  gn_forwards(g, count, issue, [&](int slot, int k) {
-    gn_write<T, ACT, CODES>(y, codes, exponents, first + k * step, kept_piece<T>(data + slot * kGnThreads, plane), c);
-  });
-}
-
-// part_channel[(image * parts + part) * 2 + {0, 1}][c] = sums of g * xhat and of g over the part's pixels;
-// part_group[(image * groups + group) * parts + part] = their weighted sums over a group's channels.
-template <class T, int ACT, bool CODES>
-__global__ void __launch_bounds__(kGnThreads, 512 / kGnThreads)
-groupnorm_2d_bwd_sums_kernel(float* __restrict__ part_channel, float2* __restrict__ part_group,
-                             const T* __restrict__ dy, const T* __restrict__ x, const uint2* __restrict__ codes,
-                             const unsigned char* __restrict__ exponents, const float2* __restrict__ stats,
-                             const float* __restrict__ weight, const float* __restrict__ bias, const GnGeom g) {
-  extern __shared__ uint4 dynamic[];
-  const GnReduce red = gn_reduce(dynamic, g);
-  GnBackRing<T, CODES> ring(dynamic, g, dy, x, codes, exponents);
-  grid_dependency_wait();
-  grid_dependency_launch_dependents();
-  const GnWork w = gn_work(g, blockIdx.x);
-  const int count = gn_count(w);
-  const long long first = gn_offset(g, w, w.px0 + w.r), step = (long long)w.rows * g.c;
-  const auto issue = [&](int slot, int k) { ring.issue(slot, first + k * step); };
-  gn_request(g, count, issue);
-  const long long first_group = gn_first_group(g, w);
-  stats += first_group;
-  GnChannels c;
-  if (w.on) gn_channels(c, g, w, gn_affine(w, weight, bias), [&](int k) { return __ldg(stats + k); });
-  GnBackSums t;
-  t.clear();
-  gn_forwards(g, count, issue,
-              [&](int slot, int k) { t.add<T, ACT>(ring.input(slot, first + k * step), ring.grad(slot), c); });
-  gn_back_groups(g, w, t, stats, weight, red, [&](int k, float2 v) {
-    if (part_group != nullptr) part_group[(first_group + k) * g.parts + w.part] = v;
-  });
-  if (part_channel != nullptr)
-    gn_back_channels(g, w, stats, red, part_channel + (w.image * g.parts + w.part) * 2 * g.c);
-}
-
-template <class T, int ACT, bool CODES>
-__global__ void __launch_bounds__(kGnThreads, 512 / kGnThreads)
-groupnorm_2d_bwd_apply_kernel(T* __restrict__ dx, const float2* __restrict__ part_group, const T* __restrict__ dy,
-                              const T* __restrict__ x, const uint2* __restrict__ codes,
-                              const unsigned char* __restrict__ exponents, const float2* __restrict__ stats,
-                              const float* __restrict__ weight, const float* __restrict__ bias, const GnGeom g) {
-  extern __shared__ uint4 dynamic[];
-  float2* inner = gn_reduce(dynamic, g).group;
-  GnBackRing<T, CODES> ring(dynamic, g, dy, x, codes, exponents);
-  const GnWork w = gn_work(g, gridDim.x - 1 - blockIdx.x);
-  const int count = gn_count(w);
-  const long long first = gn_offset(g, w, w.px0 + w.r), step = (long long)w.rows * g.c;
-  const auto issue = [&](int slot, int k) { ring.issue(slot, first + k * step); };
-  gn_request(g, count, issue);
-  grid_dependency_wait();
-  grid_dependency_launch_dependents();
-  const long long first_group = gn_first_group(g, w);
-  stats += first_group;
-  const int lane = threadIdx.x & 31;
-  for (int k = threadIdx.x >> 5; k < w.groups; k += kGnThreads / 32) {
-    float s = 0.f, q = 0.f;
-    for (int i = lane; i < g.parts; i += 32) {
-      const float2 v = __ldcg(part_group + (first_group + k) * g.parts + i);
-      s += v.x, q += v.y;
-    }
-    s = sum_lanes(s, 5), q = sum_lanes(q, 5);
-    if (lane == 0) inner[k] = gn_inner_of(make_float2(s, q), __ldg(stats + k).y, g.inv_m);
-  }
-  __syncthreads();
-  if (!w.on) return;
-  GnChannels c;
-  gn_channels(c, g, w, gn_affine(w, weight, bias), [&](int k) { return __ldg(stats + k); });
-  GnInner s;
-  gn_inner(s, g, w, [&](int k) { return inner[k]; });
-  gn_forwards(g, count, issue, [&](int slot, int k) {
-    const long long at = first + k * step;
-    store_piece(dx + at, gn_backward<T, ACT>(ring.input(slot, at), ring.grad(slot), c, s));
-  });
-}
-
-// ---------------------------------------------------------------- one launch
-//
-// The parts of a slab are the CTAs of a cluster (1 to 16) and the sums cross CTAs through distributed shared
-// memory, so one launch does both passes and the second one finds its data close by: it goes through the pieces
-// backwards, those that are still in the ring first (all of them, where a part fits), the others again from L2,
-// which holds what the resident CTAs work on many times over.
+// ---------------------------------------------------------------- sums over a cluster
 
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
@@ -871,24 +742,258 @@ __device__ __forceinline__ float2 cluster_load(const float2* p, int rank) {
   return v;
 }
 
-// Calls body(group, part, live) with the parts of a group in neighbouring lanes (parts is a power of two up
-// to 16): all lanes of a warp together, `live` where there is such a group.
+// Calls body(group, rank, live) with the CTAs of the cluster in neighbouring lanes for each group: all lanes of a warp
+// together, `live` where there is such a group.
 template <class Body>
-__device__ __forceinline__ void gn_over_parts(const GnGeom& g, const GnWork& w, Body body) {
-  const int part = threadIdx.x & (g.parts - 1), step = kGnThreads >> g.log_parts;
-  int k = threadIdx.x >> g.log_parts;
-  for (int base = 0; base < w.groups; base += step, k += step) body(k, part, k < w.groups);
+__device__ __forceinline__ void gn_over_cluster(const GnGeom& g, const GnWork& w, Body body) {
+  const int rank = threadIdx.x & (g.cluster - 1), step = kGnThreads >> g.log_cluster;
+  int k = threadIdx.x >> g.log_cluster;
+  for (int base = 0; base < w.groups; base += step, k += step) body(k, rank, k < w.groups);
 }
 
 // Every CTA of the cluster has written its `own` values (or this CTA, if it is alone).
 __device__ __forceinline__ void gn_cluster_sync(const GnGeom& g) {
-  if (g.parts > 1) {
+  if (g.cluster > 1) {
     cluster_arrive();
     cluster_wait();
   } else {
     __syncthreads();
   }
 }
+
+__device__ __forceinline__ float2 gn_of_rank(const GnGeom& g, const float2* own, int rank) {
+  return g.cluster > 1 ? cluster_load(own, rank) : *own;
+}
+
+// The groups' {mean, centred squares} over the cluster's pixels from its CTAs' own, to put(group, value) by one thread
+// each, behind gn_cluster_sync.
+template <class Put>
+__device__ __forceinline__ void gn_cluster_stats(const GnGeom& g, const GnWork& w, const float2* own, Put put) {
+  gn_over_cluster(g, w, [&](int k, int rank, bool live) {
+    const float2 v = live ? gn_of_rank(g, own + k, rank) : make_float2(0.f, 0.f);
+    GnSet set = {(float)gn_part_pixels(g, (w.part & -g.cluster) + rank) * (float)g.cpg, v.x, v.y};
+    set.merge_lanes(g.log_cluster);
+    if (live && rank == 0) put(k, make_float2(set.mean, set.m2));
+  });
+}
+
+// The groups' sums over the cluster.
+template <class Put>
+__device__ __forceinline__ void gn_cluster_sums(const GnGeom& g, const GnWork& w, const float2* own, Put put) {
+  gn_over_cluster(g, w, [&](int k, int rank, bool live) {
+    float2 v = live ? gn_of_rank(g, own + k, rank) : make_float2(0.f, 0.f);
+    v.x = sum_lanes(v.x, g.log_cluster), v.y = sum_lanes(v.y, g.log_cluster);
+    if (live && rank == 0) put(k, v);
+  });
+}
+
+// ---------------------------------------------------------------- two launches
+//
+// For a few large images: any number of CTAs works on an image, the sums go through memory (one value for each
+// cluster), and the second launch reads the input again.  It may ask for it before the first has ended (its inputs were there before that began) and
+// goes through the data backwards, so that it finds in L2 what the first launch read last.
+
+// part_stats[(image * groups + group) * clusters + cluster] = {mean, centred squares} over the cluster's pixels
+template <class T>
+__global__ void __launch_bounds__(kGnThreads, 768 / kGnThreads)
+groupnorm_2d_stats_kernel(float2* __restrict__ part_stats, const T* __restrict__ x, const GnGeom g) {
+  extern __shared__ uint4 dynamic[];
+  const GnReduce red = gn_reduce(dynamic, g);
+  constexpr int B = GnBatch<T>::forward, plane = 4 * B * kGnThreads;
+  uint4* data = reinterpret_cast<uint4*>(reinterpret_cast<char*>(dynamic) + g.data_at) + threadIdx.x;
+  grid_dependency_wait();
+  grid_dependency_launch_dependents();
+  const GnWork w = gn_work(g, blockIdx.x);
+  const int count = gn_count(w);
+  const u32 first = gn_first_piece(g, w), step = gn_step(g, w);
+  const long long start = gn_part_start(g, w);
+  x += start * 8;
+  const auto issue = [&](int slot, u32 at) { keep_piece(data + slot * kGnThreads, plane, piece_at(x, at)); };
+  gn_request<B>(count, first, step, issue);
+  GnSums t;
+  t.clear();
+  if (count > 0) t.start(values_of(load_piece(piece_at(x, first))));
+  gn_forwards<B>(count, first, step, issue, [&](int slot, u32) {
+    t.add(values_of(kept_piece<T>(data + slot * kGnThreads, plane)));
+  });
+  float2* own = red.group + g.slab_groups;
+  __syncthreads();  // the ring is free for the reductions
+  gn_group_stats(g, w, t, red, [&](int k, float2 v) { own[k] = v; });
+  gn_cluster_sync(g);
+  if ((w.part & (g.cluster - 1)) == 0) {
+    const long long first_group = gn_first_group(g, w);
+    const int clusters = g.parts >> g.log_cluster, cluster = w.part >> g.log_cluster;
+    gn_cluster_stats(g, w, own, [&](int k, float2 v) { part_stats[(first_group + k) * clusters + cluster] = v; });
+  }
+  if (g.cluster > 1) gn_cluster_sync(g);  // no CTA leaves while another reads its values
+}
+
+// Pixels of an image before part i.
+__device__ __forceinline__ int gn_part_begin(const GnGeom& g, int i) { return i * g.part_px + min(i, g.part_rest); }
+
+// body(value, cluster) for this lane's share of the clusters' values of a group.  Eight loads at a time: every CTA of
+// the second launch does this before anything else, and one load after the other took it 17 us for the 222
+// clusters of 1 x 128 x 512 x 512.
+template <class Body>
+__device__ __forceinline__ void gn_each_cluster(const float2* __restrict__ values, int clusters, Body body) {
+  const int lane = threadIdx.x & 31;
+  for (int base = 0; base < clusters; base += 256) {
+    float2 v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int i = base + j * 32 + lane;
+      v[j] = i < clusters ? __ldcg(values + i) : make_float2(0.f, 0.f);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (base + j * 32 + lane < clusters) body(v[j], base + j * 32 + lane);
+  }
+}
+
+// Mean and rstd of the slab's groups from the clusters' values, into stat[]; all threads, synchronised.
+__device__ __forceinline__ void gn_merge_parts(float2* stat, const GnGeom& g, const GnWork& w,
+                                               const float2* __restrict__ part_stats) {
+  const long long first_group = gn_first_group(g, w);
+  const int clusters = g.parts >> g.log_cluster;
+  for (int k = threadIdx.x >> 5; k < w.groups; k += kGnThreads / 32) {
+    const float2* ps = part_stats + (first_group + k) * clusters;
+    const float m0 = __ldcg(ps).x;  // (differences to one of the means: little cancels)
+    float s = 0.f, q = 0.f;
+    gn_each_cluster(ps, clusters, [&](float2 v, int i) {
+      const float n = (float)(gn_part_begin(g, (i + 1) << g.log_cluster) - gn_part_begin(g, i << g.log_cluster));
+      const float d = v.x - m0;
+      s = fmaf(n, d, s);
+      q += fmaf(n * (float)g.cpg * d, d, v.y);
+    });
+    s = sum_lanes(s, 5), q = sum_lanes(q, 5);
+    const float d = s * g.inv_pixels, m2 = not_below_zero(fmaf(-s * (float)g.cpg, d, q));
+    if ((threadIdx.x & 31) == 0) stat[k] = make_float2(m0 + d, rsqrtf(fmaf(m2, g.inv_m, g.eps)));
+  }
+  __syncthreads();
+}
+
+template <class T, int ACT, bool CODES>
+__global__ void __launch_bounds__(kGnThreads, 768 / kGnThreads)
+groupnorm_2d_apply_kernel(T* __restrict__ y, float2* __restrict__ stats, uint2* __restrict__ codes,
+                          unsigned char* __restrict__ exponents, const T* __restrict__ x,
+                          const float* __restrict__ weight, const float* __restrict__ bias,
+                          const float2* __restrict__ part_stats, const GnGeom g) {
+  extern __shared__ uint4 dynamic[];
+  float2* stat = gn_reduce(dynamic, g).group;
+  constexpr int B = GnBatch<T>::forward, plane = 4 * B * kGnThreads;
+  uint4* data = reinterpret_cast<uint4*>(reinterpret_cast<char*>(dynamic) + g.data_at) + threadIdx.x;
+  const GnWork w = gn_work(g, gridDim.x - 1 - blockIdx.x);
+  const int count = gn_count(w);
+  const u32 first = gn_first_piece(g, w), step = gn_step(g, w);
+  const long long start = gn_part_start(g, w);
+  x += start * 8;
+  y += start * 8;
+  if (CODES) codes += start, exponents += start;
+  const auto issue = [&](int slot, u32 at) { keep_piece(data + slot * kGnThreads, plane, piece_at(x, at)); };
+  gn_request<B>(count, first, step, issue);
+  grid_dependency_wait();
+  grid_dependency_launch_dependents();
+  gn_merge_parts(stat, g, w, part_stats);
+  if (stats != nullptr && w.part == 0) {
+    for (int k = threadIdx.x; k < w.groups; k += kGnThreads) stats[gn_first_group(g, w) + k] = stat[k];
+  }
+  if (!w.on) return;
+  GnChannels c;
+  gn_channels(c, g, w, gn_affine(w, weight, bias), [&](int k) { return stat[k]; });
+  gn_forwards<B>(count, first, step, issue, [&](int slot, u32 at) {
+    gn_write<T, ACT, CODES>(y, codes, exponents, at, kept_piece<T>(data + slot * kGnThreads, plane), c);
+  });
+}
+
+// part_channel[(image * parts + part) * 2 + {0, 1}][c] = sums of g * xhat and of g over the part's pixels;
+// part_group[(image * groups + group) * clusters + cluster] = their weighted sums over a group's channels and the
+// cluster's pixels.
+template <class T, int ACT, bool CODES>
+__global__ void __launch_bounds__(kGnThreads, 512 / kGnThreads)
+groupnorm_2d_bwd_sums_kernel(float* __restrict__ part_channel, float2* __restrict__ part_group,
+                             const T* __restrict__ dy, const T* __restrict__ x, const uint2* __restrict__ codes,
+                             const unsigned char* __restrict__ exponents, const float2* __restrict__ stats,
+                             const float* __restrict__ weight, const float* __restrict__ bias, const GnGeom g) {
+  extern __shared__ uint4 dynamic[];
+  const GnReduce red = gn_reduce(dynamic, g);
+  grid_dependency_wait();
+  grid_dependency_launch_dependents();
+  const GnWork w = gn_work(g, blockIdx.x);
+  const int count = gn_count(w);
+  const u32 first = gn_first_piece(g, w), step = gn_step(g, w);
+  const long long start = gn_part_start(g, w);
+  GnBackRing<T, CODES> ring(dynamic, g, start, dy, x, codes, exponents);
+  const auto issue = [&](int slot, u32 at) { ring.issue(slot, at); };
+  constexpr int B = GnBatch<T>::backward;
+  gn_request<B>(count, first, step, issue);
+  const long long first_group = gn_first_group(g, w);
+  stats += first_group;
+  GnChannels c;
+  if (w.on) gn_channels(c, g, w, gn_affine(w, weight, bias), [&](int k) { return __ldg(stats + k); });
+  GnBackSums t;
+  t.clear();
+  gn_forwards<B>(count, first, step, issue,
+                 [&](int slot, u32 at) { t.add<T, ACT>(ring.input(slot, at), ring.grad(slot), c); });
+  float2* own = red.group + g.slab_groups;
+  __syncthreads();  // the ring is free for the reductions
+  gn_back_groups(g, w, t, stats, weight, red, [&](int k, float2 v) { own[k] = v; });
+  if (g.cluster > 1) cluster_arrive();
+  if (part_channel != nullptr)
+    gn_back_channels(g, w, stats, red, part_channel + (w.image * g.parts + w.part) * 2 * g.c);
+  if (g.cluster > 1) cluster_wait();
+  else __syncthreads();
+  if (part_group != nullptr && (w.part & (g.cluster - 1)) == 0) {
+    const int clusters = g.parts >> g.log_cluster, cluster = w.part >> g.log_cluster;
+    gn_cluster_sums(g, w, own, [&](int k, float2 v) { part_group[(first_group + k) * clusters + cluster] = v; });
+  }
+  if (g.cluster > 1) gn_cluster_sync(g);
+}
+
+template <class T, int ACT, bool CODES>
+__global__ void __launch_bounds__(kGnThreads, 512 / kGnThreads)
+groupnorm_2d_bwd_apply_kernel(T* __restrict__ dx, const float2* __restrict__ part_group, const T* __restrict__ dy,
+                              const T* __restrict__ x, const uint2* __restrict__ codes,
+                              const unsigned char* __restrict__ exponents, const float2* __restrict__ stats,
+                              const float* __restrict__ weight, const float* __restrict__ bias, const GnGeom g) {
+  extern __shared__ uint4 dynamic[];
+  float2* inner = gn_reduce(dynamic, g).group;
+  const GnWork w = gn_work(g, gridDim.x - 1 - blockIdx.x);
+  const int count = gn_count(w);
+  const u32 first = gn_first_piece(g, w), step = gn_step(g, w);
+  const long long start = gn_part_start(g, w);
+  GnBackRing<T, CODES> ring(dynamic, g, start, dy, x, codes, exponents);
+  dx += start * 8;
+  const auto issue = [&](int slot, u32 at) { ring.issue(slot, at); };
+  constexpr int B = GnBatch<T>::backward;
+  gn_request<B>(count, first, step, issue);
+  grid_dependency_wait();
+  grid_dependency_launch_dependents();
+  const long long first_group = gn_first_group(g, w);
+  stats += first_group;
+  const int clusters = g.parts >> g.log_cluster;
+  for (int k = threadIdx.x >> 5; k < w.groups; k += kGnThreads / 32) {
+    float s = 0.f, q = 0.f;
+    gn_each_cluster(part_group + (first_group + k) * clusters, clusters, [&](float2 v, int) { s += v.x, q += v.y; });
+    s = sum_lanes(s, 5), q = sum_lanes(q, 5);
+    if ((threadIdx.x & 31) == 0) inner[k] = gn_inner_of(make_float2(s, q), __ldg(stats + k).y, g.inv_m);
+  }
+  __syncthreads();
+  if (!w.on) return;
+  GnChannels c;
+  gn_channels(c, g, w, gn_affine(w, weight, bias), [&](int k) { return __ldg(stats + k); });
+  GnInner s;
+  gn_inner(s, g, w, [&](int k) { return inner[k]; });
+  gn_forwards<B>(count, first, step, issue, [&](int slot, u32 at) {
+    store_piece(piece_at(dx, at), gn_backward<T, ACT>(ring.input(slot, at), ring.grad(slot), c, s));
+  });
+}
+
+// ---------------------------------------------------------------- one launch
+//
+// The parts of a slab are the CTAs of a cluster (1 to 16) and the sums cross CTAs through distributed shared
+// memory, so one launch does both passes and the second one finds its data close by: it goes through the pieces
+// backwards, those that are still in the ring first (all of them, where a part fits), the others again from L2,
+// which holds what the resident CTAs work on many times over.
 
 template <class T, int ACT, bool CODES>
 __global__ void __launch_bounds__(kGnThreads, 768 / kGnThreads)
@@ -899,52 +1004,44 @@ groupnorm_2d_fwd_kernel(T* __restrict__ y, float2* __restrict__ stats, uint2* __
   const GnReduce red = gn_reduce(dynamic, g);
   float2* own = red.group + g.slab_groups;
   float2* stat = own + g.slab_groups;
-  const int plane = g.slots * kGnThreads;
+  constexpr int B = GnBatch<T>::forward, plane = 4 * B * kGnThreads;
   uint4* data = reinterpret_cast<uint4*>(reinterpret_cast<char*>(dynamic) + g.data_at) + threadIdx.x;
 
   grid_dependency_wait();
   grid_dependency_launch_dependents();
   const GnWork w = gn_work(g, blockIdx.x);
   const int count = gn_count(w);
-  const long long first = gn_offset(g, w, w.px0 + w.r), step = (long long)w.rows * g.c;
-  const auto issue = [&](int slot, int k) { keep_piece(data + slot * kGnThreads, plane, x + first + k * step); };
-  gn_request(g, count, issue);
-  float origin[8];
-  gn_origin(origin, g, w, x);
+  const u32 first = gn_first_piece(g, w), step = gn_step(g, w);
+  const long long start = gn_part_start(g, w);
+  x += start * 8;
+  y += start * 8;
+  if (CODES) codes += start, exponents += start;
+  const auto issue = [&](int slot, u32 at) { keep_piece(data + slot * kGnThreads, plane, piece_at(x, at)); };
+  gn_request<B>(count, first, step, issue);
   GnSums t;
   t.clear();
-  if (count > 0) t.start(values_of(load_piece(x + first)));
-  gn_forwards(g, count, issue,
-              [&](int slot, int) { t.add(values_of(kept_piece<T>(data + slot * kGnThreads, plane))); });
-  gn_group_stats(g, w, t, origin, red, [&](int k, float2 v) { own[k] = v; });
+  if (count > 0) t.start(values_of(load_piece(piece_at(x, first))));
+  gn_forwards<B>(count, first, step, issue, [&](int slot, u32) {
+    t.add(values_of(kept_piece<T>(data + slot * kGnThreads, plane)));
+  });
+  gn_group_stats(g, w, t, red, [&](int k, float2 v) { own[k] = v; });
   const GnAffine affine = w.on ? gn_affine(w, weight, bias) : GnAffine();  // (on its way across the barrier)
   gn_cluster_sync(g);
-  gn_over_parts(g, w, [&](int k, int part, bool live) {
-    const float2 v = live ? (g.parts > 1 ? cluster_load(own + k, part) : own[k]) : make_float2(0.f, 0.f);
-    const float n = (float)gn_part_pixels(g, part);
-    float mean = v.x, m2 = v.y;
-    if (g.parts > 1) {
-      const float m0 = __shfl_sync(0xffffffffu, v.x, 0, g.parts);
-      mean = fmaf(sum_lanes(live ? n * (v.x - m0) : 0.f, g.log_parts), g.inv_pixels, m0);
-      const float d = v.x - mean;
-      m2 = sum_lanes(fmaf(n * (float)g.cpg * d, d, v.y), g.log_parts);
-    }
-    if (live && part == 0) {
-      const float2 st = make_float2(mean, rsqrtf(fmaf(m2, g.inv_m, g.eps)));
-      stat[k] = st;
-      if (stats != nullptr && w.part == 0) stats[gn_first_group(g, w) + k] = st;
-    }
+  gn_cluster_stats(g, w, own, [&](int k, float2 v) {
+    const float2 st = make_float2(v.x, rsqrtf(fmaf(not_below_zero(v.y), g.inv_m, g.eps)));
+    stat[k] = st;
+    if (stats != nullptr && w.part == 0) stats[gn_first_group(g, w) + k] = st;
   });
-  if (g.parts > 1) cluster_arrive();  // (this CTA has read the others' values; waited for at the end)
+  if (g.cluster > 1) cluster_arrive();  // (this CTA has read the others' values; waited for at the end)
   __syncthreads();
   if (w.on) {
     GnChannels c;
     gn_channels(c, g, w, affine, [&](int k) { return stat[k]; });
-    gn_backwards(g, count, issue, [&](int slot, int k) {
-      gn_write<T, ACT, CODES>(y, codes, exponents, first + k * step, kept_piece<T>(data + slot * kGnThreads, plane), c);
+    gn_backwards<B>(g.batches, count, first, step, issue, [&](int slot, u32 at) {
+      gn_write<T, ACT, CODES>(y, codes, exponents, at, kept_piece<T>(data + slot * kGnThreads, plane), c);
     });
   }
-  if (g.parts > 1) cluster_wait();  // no CTA leaves while another reads its values
+  if (g.cluster > 1) cluster_wait();  // no CTA leaves while another reads its values
 }
 
 // part_channel as of groupnorm_2d_bwd_sums_kernel; dx may be NULL.
@@ -958,42 +1055,40 @@ groupnorm_2d_bwd_kernel(T* __restrict__ dx, float* __restrict__ part_channel, co
   const GnReduce red = gn_reduce(dynamic, g);
   float2* own = red.group + g.slab_groups;
   float2* inner = own + g.slab_groups;
-  GnBackRing<T, CODES> ring(dynamic, g, dy, x, codes, exponents);
   grid_dependency_wait();
   grid_dependency_launch_dependents();
   const GnWork w = gn_work(g, blockIdx.x);
   const int count = gn_count(w);
-  const long long first = gn_offset(g, w, w.px0 + w.r), step = (long long)w.rows * g.c;
-  const auto issue = [&](int slot, int k) { ring.issue(slot, first + k * step); };
-  gn_request(g, count, issue);
+  const u32 first = gn_first_piece(g, w), step = gn_step(g, w);
+  const long long start = gn_part_start(g, w);
+  GnBackRing<T, CODES> ring(dynamic, g, start, dy, x, codes, exponents);
+  if (dx != nullptr) dx += start * 8;
+  const auto issue = [&](int slot, u32 at) { ring.issue(slot, at); };
+  constexpr int B = GnBatch<T>::backward;
+  gn_request<B>(count, first, step, issue);
   stats += gn_first_group(g, w);
   GnChannels c;
   if (w.on) gn_channels(c, g, w, gn_affine(w, weight, bias), [&](int k) { return __ldg(stats + k); });
   GnBackSums t;
   t.clear();
-  gn_forwards(g, count, issue,
-              [&](int slot, int k) { t.add<T, ACT>(ring.input(slot, first + k * step), ring.grad(slot), c); });
+  gn_forwards<B>(count, first, step, issue,
+                 [&](int slot, u32 at) { t.add<T, ACT>(ring.input(slot, at), ring.grad(slot), c); });
   gn_back_groups(g, w, t, stats, weight, red, [&](int k, float2 v) { own[k] = v; });
-  if (g.parts > 1) cluster_arrive();
+  if (g.cluster > 1) cluster_arrive();
   if (part_channel != nullptr) gn_back_channels(g, w, stats, red, part_channel + (w.image * g.parts + w.part) * 2 * g.c);
-  if (g.parts > 1) cluster_wait();
+  if (g.cluster > 1) cluster_wait();
   else __syncthreads();
-  gn_over_parts(g, w, [&](int k, int part, bool live) {
-    float2 v = live ? (g.parts > 1 ? cluster_load(own + k, part) : own[k]) : make_float2(0.f, 0.f);
-    v.x = sum_lanes(v.x, g.log_parts), v.y = sum_lanes(v.y, g.log_parts);
-    if (live && part == 0) inner[k] = gn_inner_of(v, __ldg(stats + k).y, g.inv_m);
-  });
-  if (g.parts > 1) cluster_arrive();
+  gn_cluster_sums(g, w, own, [&](int k, float2 v) { inner[k] = gn_inner_of(v, __ldg(stats + k).y, g.inv_m); });
+  if (g.cluster > 1) cluster_arrive();
   __syncthreads();
   if (w.on && dx != nullptr) {
     GnInner s;
     gn_inner(s, g, w, [&](int k) { return inner[k]; });
-    gn_backwards(g, count, issue, [&](int slot, int k) {
-      const long long at = first + k * step;
-      store_piece(dx + at, gn_backward<T, ACT>(ring.input(slot, at), ring.grad(slot), c, s));
+    gn_backwards<B>(g.batches, count, first, step, issue, [&](int slot, u32 at) {
+      store_piece(piece_at(dx, at), gn_backward<T, ACT>(ring.input(slot, at), ring.grad(slot), c, s));
     });
   }
-  if (g.parts > 1) cluster_wait();
+  if (g.cluster > 1) cluster_wait();
 }
 
 }  // namespace GN_NAMESPACE

@@ -29,9 +29,10 @@ struct GnGeom {
   int fold, lanes, run, run_rows, run_rest, column_lanes;
   float inv_run;
   int slab_groups;  // of a full slab
-  int group_at;     // where the groups' values start in the dynamic shared memory
-  // one launch: log2(parts), slots of a thread's ring and of a quarter of it, quarters of a part, where the ring is
-  int log_parts, slots, batch, batches, data_at;
+  int plane;        // values of one of the reductions' arrays
+  int planes_at, group_at;  // where these and the groups' values start in the dynamic shared memory
+  int cluster, log_cluster;  // CTAs of a cluster, a power of two that divides parts
+  int batches, data_at;      // batches of pieces of a thread, where the ring is
 };
 
 struct GnKernels {

@@ -1,5 +1,7 @@
 """The 8-bit form of activations and the convolution that keeps its input in it."""
 
+import gc
+
 import pytest
 import torch
 
@@ -170,6 +172,7 @@ def test_memory_kept_for_the_backward_pass():
     w = torch.randn(64, 8, 3, 3, device="cuda").half().requires_grad_(True)
     kept = []
     for conv in (conv2d_gw8, conv2d_gw8_checkpoint8):
+        gc.collect()      # what earlier tests left in cycles is not to be freed in between
         torch.cuda.synchronize()
         before = torch.cuda.memory_allocated()
         x = torch.randn(sh.n, sh.c, sh.h, sh.w, device="cuda").half().contiguous(memory_format=CL)

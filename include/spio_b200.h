@@ -348,7 +348,9 @@ int spio_layernorm_2d_bwd(void* dx, float* dweight, float* dbias, const void* dy
  *   bwd: dx (NULL: not wanted), dweight and dbias (fp32 [c], NULL: not wanted) from dy, stats and
  *        either x or, if codes and exponents are given, the values they stand for; sums are added in
  *        a fixed order.  bias is needed where the activation has a slope.
- * scratch is device memory of at least the given size, 16-byte aligned; its contents do not matter. */
+ * Tensors are 16-byte aligned, codes and stats 8-byte, exponents 4-byte.  scratch is device memory of at least
+ * the size that the call before it gives for the descriptor on the current device (which may be 0: NULL will do),
+ * 16-byte aligned; its contents do not matter. */
 enum { SPIO_TYPE_F16 = 0, SPIO_TYPE_BF16 = 1, SPIO_TYPE_F32 = 2 };
 enum { SPIO_ACT_NONE = 0, SPIO_ACT_RELU = 1, SPIO_ACT_SILU = 2, SPIO_ACT_GELU = 3 };
 typedef struct spio_groupnorm_2d_desc {

@@ -5,6 +5,7 @@
 #include <algorithm>
 #include <array>
 #include <cmath>
+#include <exception>
 #include <map>
 #include <mutex>
 #include <numeric>
@@ -285,15 +286,19 @@ int make_plan(const spio_groupnorm_2d_desc* d, const Device& dev, bool backward,
   static std::map<Key, Plan> plans;
   const Key key = {d->n, d->pixels, d->c, d->groups, d->type * 16 + d->activation, backward * 2 + coded,
                    (long long)dev.sms << 32 | dev.smem};
-  std::lock_guard<std::mutex> lock(mutex);
-  auto it = plans.find(key);
-  if (it == plans.end()) {
-    Plan fresh;
-    if (choose_plan(d, dev, backward, coded, &fresh)) return 1;
-    if (plans.size() >= 4096) plans.clear();
-    it = plans.insert_or_assign(key, fresh).first;
+  try {
+    std::lock_guard<std::mutex> lock(mutex);
+    auto it = plans.find(key);
+    if (it == plans.end()) {
+      Plan fresh;
+      if (choose_plan(d, dev, backward, coded, &fresh)) return 1;
+      if (plans.size() >= 4096) plans.clear();
+      it = plans.insert_or_assign(key, fresh).first;
+    }
+    *p = it->second;
+  } catch (const std::exception& e) {  // no memory; C callers get an error like any other
+    return jit_fail(std::string("GroupNorm2d: ") + e.what());
   }
-  *p = it->second;
   p->g.eps = d->eps;
   return 0;
 }
@@ -342,10 +347,10 @@ extern "C" {
 
 size_t spio_groupnorm_2d_fwd_scratch_bytes(const spio_groupnorm_2d_desc* desc) {
   Device dev;
-  Plan p;
+  Plan p, q;
   if (check_desc(desc) || desc->n == 0 || desc->pixels == 0) return 0;
-  if (device_of(&dev) || make_plan(desc, dev, false, false, &p)) return 0;
-  return p.stats_bytes;
+  if (device_of(&dev) || make_plan(desc, dev, false, false, &p) || make_plan(desc, dev, false, true, &q)) return 0;
+  return std::max(p.stats_bytes, q.stats_bytes);
 }
 
 int spio_groupnorm_2d_fwd(void* y, float* stats, void* codes, void* exponents, const void* x, const float* weight,

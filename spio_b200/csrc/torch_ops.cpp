@@ -115,7 +115,7 @@ spio_groupnorm_2d_desc describe(const Tensor& x, const OptTensor& weight, const 
   TORCH_CHECK_VALUE(c <= (1 << 20), "GroupNorm2d supports at most 2^20 channels");
   TORCH_CHECK_VALUE(eps >= 0, "eps must not be negative");
   for (const OptTensor* t : {&weight, &bias})
-    TORCH_CHECK_VALUE(!t->has_value() || ((*t)->scalar_type() == at::kFloat && (*t)->numel() == c && (*t)->device() == x.device()),
+    TORCH_CHECK_VALUE(!t->has_value() || ((*t)->scalar_type() == at::kFloat && (*t)->dim() == 1 && (*t)->numel() == c && (*t)->device() == x.device()),
                       "weight and bias are fp32 vectors of the channels on the data's device");
   spio_groupnorm_2d_desc d;
   d.n = x.size(0);
@@ -269,8 +269,17 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
 
 bool requires_grad(const OptTensor& t) { return t.has_value() && t->requires_grad(); }
 
+// Forward-mode derivatives: refused, or the result would seem constant.
+void check_no_tangent(const Tensor& t) {
+  TORCH_CHECK(!t._fw_grad(0).defined(), "spio groupnorm_2d has no forward-mode derivative");
+}
+void check_no_tangent(const OptTensor& t) {
+  if (t.has_value()) check_no_tangent(*t);
+}
+
 Tensor groupnorm_2d_autograd(const Tensor& x, const OptTensor& weight, const OptTensor& bias, int64_t num_groups,
                              double eps, c10::string_view activation, bool checkpoint8) {
+  check_no_tangent(x), check_no_tangent(weight), check_no_tangent(bias);
   if (at::GradMode::is_enabled() && (x.requires_grad() || requires_grad(weight) || requires_grad(bias)))
     return GroupNorm::apply(x, weight, bias, num_groups, eps, std::string(activation), checkpoint8);
   at::AutoDispatchBelowADInplaceOrView below;
@@ -298,6 +307,7 @@ std::tuple<Tensor, Tensor, Tensor> groupnorm_2d_backward_autograd(
     const Tensor& dy, const OptTensor& x, const OptTensor& codes, const OptTensor& exponents, const Tensor& stats,
     const OptTensor& weight, const OptTensor& bias, int64_t num_groups, c10::string_view activation,
     bool needs_input_grad, bool needs_weight_grad, bool needs_bias_grad) {
+  check_no_tangent(dy), check_no_tangent(x), check_no_tangent(weight), check_no_tangent(bias);
   if (at::GradMode::is_enabled() && (dy.requires_grad() || requires_grad(x) || requires_grad(weight) || requires_grad(bias))) {
     const variable_list r =
         GroupNormBackward::apply(dy, x, codes, exponents, stats, weight, bias, num_groups, std::string(activation),

@@ -70,8 +70,9 @@ def groupnorm_2d(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor
     """``activation(group_norm(x))`` of an NCHW tensor (channels_last on a CUDA device; float16, bfloat16 or
     float32, a multiple of 8 channels).
 
-    ``weight`` and ``bias`` are fp32 vectors of the channels (of any type under autocast); ``activation`` is
-    ``"none"``, ``"relu"``, ``"silu"`` or ``"gelu"`` (with the error function).  ``checkpoint8`` keeps the 8-bit form of
+    ``weight`` and ``bias`` are fp32 vectors of the channels (of any type under autocast, where the data keeps its
+    own); ``activation`` is ``"none"``, ``"relu"``, ``"silu"`` or ``"gelu"`` (with the error function).  A group, rounded
+    up to whole blocks of 8 channels, may span at most 2048 channels.  ``checkpoint8`` keeps the 8-bit form of
     ``x`` for the backward pass instead of ``x`` (1.125 bytes a value): the gradients are then taken at the
     restored values, with the statistics of ``x`` itself."""
     _clib.load_torch_ops()

@@ -3,6 +3,7 @@
 
 from __future__ import annotations
 
+import math
 from typing import Optional
 
 import torch
@@ -11,14 +12,21 @@ from torch import nn
 from ..functional.groupnorm_2d_function import ACTIVATIONS, groupnorm_2d
 
 
+def _fits(num_groups: int, num_channels: int) -> bool:
+    """The kernels hold whole groups and whole blocks of 8 channels in one thread block."""
+    return math.lcm(num_channels // num_groups, 8) <= 2048
+
+
 class GroupNorm2d(nn.Module):
     """``activation(group_norm(x))``; ``checkpoint8`` keeps the input in 8 bits for the backward pass."""
 
     def __init__(self, num_groups: int, num_channels: int, eps: float = 1e-5, affine: bool = True,
                  activation: str = "none", checkpoint8: bool = False, device=None, dtype=torch.float32):
         super().__init__()
-        if num_channels % 8 != 0 or num_groups <= 0 or num_channels % num_groups != 0:
+        if num_channels <= 0 or num_channels % 8 != 0 or num_groups <= 0 or num_channels % num_groups != 0:
             raise ValueError("GroupNorm2d needs a multiple of 8 channels that the number of groups divides")
+        if not _fits(num_groups, num_channels):
+            raise ValueError("GroupNorm2d: groups (rounded up to whole blocks of 8 channels) may span at most 2048 channels")
         if activation not in ACTIVATIONS:
             raise ValueError(f"activation must be one of {', '.join(ACTIVATIONS)}")
         self.num_groups = num_groups
@@ -37,7 +45,8 @@ class GroupNorm2d(nn.Module):
     @staticmethod
     def match(module: nn.Module) -> bool:
         """True for an ``nn.GroupNorm`` that this layer can replace when it is applied to an image tensor."""
-        return isinstance(module, nn.GroupNorm) and module.num_channels % 8 == 0
+        return (isinstance(module, nn.GroupNorm) and module.num_channels % 8 == 0
+                and _fits(module.num_groups, module.num_channels))
 
     @staticmethod
     def activation_of(module: Optional[nn.Module]) -> Optional[str]:

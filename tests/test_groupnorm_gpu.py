@@ -194,6 +194,33 @@ def test_second_derivatives_are_refused():
         dx.square().sum().backward()
 
 
+@pytest.mark.parametrize("shape,groups,act,dtype", [((4, 24, 144, 122), 2, "relu", torch.float16),
+                                                    ((2, 8, 223, 200), 1, "none", torch.float32)], ids=str)
+def test_sizes_where_only_the_checkpoint_takes_two_launches(shape, groups, act, dtype):
+    """(On a B200.)  The scratch memory has to serve the form that needs more of it."""
+    for checkpoint8 in (False, True):
+        check_all(shape, groups, dtype, act, checkpoint8, seed=18)
+
+
+def test_forward_mode_derivatives_are_refused():
+    x, dy, w, b = make((2, 16, 4, 4), torch.float32, seed=19)
+    stats = groupnorm_2d_op(x, w, b, 4, 1e-5, "none", False)[1]
+    with torch.autograd.forward_ad.dual_level():
+        dual = lambda t: torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: groupnorm_2d(dual(x), 4, w, b), lambda: groupnorm_2d(x, 4, dual(w), b),
+                     lambda: groupnorm_2d(x, 4, w, dual(b)),
+                     lambda: groupnorm_2d_backward_op(dual(dy), x, None, None, stats, w, b, 4, "none", True, True, True)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+
+
+def test_functional_transforms_are_refused():
+    """(As they are by the other operators of the package.)"""
+    x, _, w, b = make((2, 16, 4, 4), torch.float32, seed=20)
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda x: groupnorm_2d(x, 4, w, b, activation="gelu").sum())(x)
+
+
 def test_compiled_model_traces_through_the_operator():
     """torch.compile sees one opaque operator (eager backend: nothing else is compiled)."""
     x, _, w, b = make((2, 32, 6, 6), torch.float16, seed=17)
@@ -299,6 +326,7 @@ def test_refusals():
         lambda: groupnorm_2d(x, 4, w.half(), b),
         lambda: groupnorm_2d(x, 4, w[:16], b),
         lambda: groupnorm_2d(x, 4, w.cpu(), b),
+        lambda: groupnorm_2d(x, 4, w.view(1, 32, 1, 1), b),
         lambda: groupnorm_2d(x, 4, activation="tanh"),
         lambda: groupnorm_2d(x, 4, eps=-1.0),
         lambda: groupnorm_2d(torch.zeros(1, 4096, 1, 1, device="cuda"), 1),
@@ -311,6 +339,8 @@ def test_refusals():
         GroupNorm2d(3, 32)
     with pytest.raises(ValueError):
         GroupNorm2d(4, 36)
+    with pytest.raises(ValueError):
+        GroupNorm2d(1, 4096)
 
 
 def test_offsets_beyond_32_bits():

@@ -41,7 +41,7 @@ def test_library_refuses_pointers():
     for args, message in [((None, None, None, None, 16), "NULL"), ((16, None, None, None, None), "NULL"),
                           ((24, None, None, None, 16), "16-byte"), ((16, None, None, None, 8), "16-byte"),
                           ((16, 4, None, None, 16), "8-byte"), ((16, None, 16, None, 16), "together"),
-                          ((16, None, 12, 16, 16), "8-byte")]:
+                          ((16, None, 12, 16, 16), "8-byte"), ((16, None, 16, 18, 16), "4-byte")]:
         assert fwd(*args, None, None, desc(), 16, 1 << 20, None) != 0 and message in _clib.last_error(), args
     for args, message in [((16, None, None, None, 16, None, None, 16), "NULL"), ((16, None, None, 16, None, None, None, 16), "NULL"),
                           ((16, None, None, 16, 16, None, None, None), "NULL"), ((8, None, None, 16, 16, None, None, 16), "16-byte"),
@@ -85,7 +85,7 @@ def test_shapes_under_fake_tensors():
 
 def test_module_matching():
     assert GroupNorm2d.match(nn.GroupNorm(4, 32)) and not GroupNorm2d.match(nn.GroupNorm(4, 36))
-    assert not GroupNorm2d.match(nn.BatchNorm2d(32))
+    assert not GroupNorm2d.match(nn.BatchNorm2d(32)) and not GroupNorm2d.match(nn.GroupNorm(1, 4096))
     gn = GroupNorm2d.from_torch_module(nn.GroupNorm(4, 32, eps=1e-3, affine=False).eval(), "gelu", True)
     assert gn.weight is None and gn.eps == 1e-3 and gn.checkpoint8 and not gn.training
     assert [GroupNorm2d.activation_of(m) for m in (nn.ReLU(), nn.SiLU(), nn.GELU(), nn.GELU("tanh"), nn.Tanh())] == [

@@ -91,6 +91,8 @@ def main() -> None:
     ap = argparse.ArgumentParser()
     ap.add_argument("--batch", type=int, default=256)
     ap.add_argument("--steps", type=int, default=5)
+    ap.add_argument("--checkpoint8", action="store_true",
+                    help="keep the inputs of the swapped convolutions in 8 bits for the backward pass")
     args = ap.parse_args()
     torch.manual_seed(1234 + 4)
     dev = torch.device("cuda")
@@ -99,10 +101,10 @@ def main() -> None:
     labels = torch.randint(0, 1000, (args.batch,), device=dev)
     import copy
 
-    fast, replaced = _transform(model)
+    fast, replaced = _transform(model, checkpoint8=args.checkpoint8)
     with_ln = copy.deepcopy(model)
     n_ln = swap_layernorm(with_ln)          # before tracing: transform keeps the fused modules
-    fused, _ = _transform(with_ln)
+    fused, _ = _transform(with_ln, checkpoint8=args.checkpoint8)
     for name, net in (("torch / cuDNN grouped conv", model), (f"spio_b200 ({replaced} layers swapped)", fast),
                       (f"spio_b200 ({replaced} convs + {n_ln} LayerNorm2d swapped)", fused)):
         for _ in range(2):

@@ -19,6 +19,7 @@ from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
+from torch.overrides import handle_torch_function, has_torch_function
 
 from .. import _clib
 from ..compiler import flags
@@ -60,6 +61,8 @@ def _checkpoint8_unpack_fake(codes, exponents, dtype):
 def checkpoint8_pack(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """The 8-bit form of an NCHW tensor (channels_last, a multiple of 8 channels; float16, bfloat16 or float32):
     ``(codes int8 (n, c, h, w), exponents uint8 (n, c / 8, h, w))``, both channels_last.  Not differentiable."""
+    if has_torch_function((x,)):      # a torch.fx proxy, a tensor subclass
+        return handle_torch_function(checkpoint8_pack, (x,), x)
     _clib.load_torch_ops()
     return _pack(x.detach() if x.requires_grad else x)
 
@@ -164,6 +167,9 @@ def conv2d_gw8_checkpoint8(inputs: torch.Tensor, weight: torch.Tensor, bias: Opt
     """:func:`conv2d_gw8` that keeps the 8-bit form of ``inputs`` for the backward pass (1.125 bytes a value
     instead of 2).  Output, input gradient and bias gradient are those of :func:`conv2d_gw8`; the weight gradient
     is taken at the restored input."""
+    if has_torch_function((inputs, weight, bias)):      # a torch.fx proxy, a tensor subclass
+        return handle_torch_function(conv2d_gw8_checkpoint8, (inputs, weight, bias), inputs, weight, bias, stride=stride,
+                                     padding_y=padding_y, padding_x=padding_x, dilation=dilation, groups=groups)
     _clib.load_torch_ops()
     if torch.is_grad_enabled() and weight.requires_grad:
         tunes = _eager_tunes(inputs, weight, bias, stride, padding_y, padding_x, dilation, groups)

@@ -90,6 +90,8 @@ def test_layouts_and_empty_tensors():
     assert torch.equal(checkpoint8_unpack(b[0].contiguous(), b[1].contiguous()), back)     # NCHW order of both
     off = torch.empty(x.numel() + 1, device="cuda", dtype=x.dtype)[1:].view(2, 5, 6, 16).permute(0, 3, 1, 2).copy_(x)
     assert torch.equal(checkpoint8_pack(off)[0], b[0])
+    odd = torch.empty(b[1].numel() + 1, device="cuda", dtype=torch.uint8)[1:].view(2, 5, 6, 2).permute(0, 3, 1, 2).copy_(b[1])
+    assert torch.equal(checkpoint8_unpack(b[0], odd), back)                               # exponents at an odd address
     codes, exponents = checkpoint8_pack(x[:0])
     assert codes.shape == (0, 16, 5, 6) and exponents.shape == (0, 2, 5, 6)
     assert checkpoint8_unpack(codes, exponents).shape == (0, 16, 5, 6)
@@ -164,6 +166,27 @@ def test_convolution_under_autocast_and_with_frozen_parts():
     (dx,) = torch.autograd.grad(y, xd, dy.cuda())
     (rx,) = torch.autograd.grad(conv2d_gw8(xd, wd, None, 1, 1, 1, 1, sh.groups), xd, dy.cuda())
     assert torch.equal(dx, rx)
+
+
+def test_second_derivatives_are_refused():
+    sh = CONVS[0]
+    x, w, _, dy = O.make_inputs(sh, seed=33, bias=False)
+    xd, wd = x.cuda().requires_grad_(True), w.cuda().requires_grad_(True)
+    y = conv2d_gw8_checkpoint8(xd, wd, None, padding_y=1, padding_x=1, groups=sh.groups)
+    with pytest.raises(RuntimeError, match="twice"):
+        torch.autograd.grad(y, (xd, wd), dy.cuda(), create_graph=True)
+
+
+def test_compiled_calls():
+    """They take the Python operator: the same values as the plain eager calls."""
+    sh = CONVS[0]
+    x, w, b, dy = (t.cuda() for t in O.make_inputs(sh, seed=34))
+    f = lambda x, w: (conv2d_gw8_checkpoint8(x, w, b, padding_y=1, padding_x=1, groups=sh.groups) * dy).sum()  # noqa: E731
+    leaves = [t.clone().requires_grad_(True) for t in (x, w)]
+    want = torch.autograd.grad(f(*leaves), leaves)
+    compiled = torch.compile(f, backend="aot_eager", fullgraph=True)
+    got = torch.autograd.grad(compiled(*leaves), leaves)
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
 
 
 def test_memory_kept_for_the_backward_pass():

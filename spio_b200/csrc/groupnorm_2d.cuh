@@ -731,6 +731,8 @@ struct GnBackRing {
 // ---------------------------------------------------------------- sums over a cluster
 
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+// (by threads that have nothing to show, only read)
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 
 // *p of the CTA `rank` of the cluster
@@ -1032,7 +1034,7 @@ groupnorm_2d_fwd_kernel(T* __restrict__ y, float2* __restrict__ stats, uint2* __
     stat[k] = st;
     if (stats != nullptr && w.part == 0) stats[gn_first_group(g, w) + k] = st;
   });
-  if (g.cluster > 1) cluster_arrive();  // (this CTA has read the others' values; waited for at the end)
+  if (g.cluster > 1) cluster_arrive_relaxed();  // (this CTA has read the others' values; waited for at the end)
   __syncthreads();
   if (w.on) {
     GnChannels c;
@@ -1079,7 +1081,7 @@ groupnorm_2d_bwd_kernel(T* __restrict__ dx, float* __restrict__ part_channel, co
   if (g.cluster > 1) cluster_wait();
   else __syncthreads();
   gn_cluster_sums(g, w, own, [&](int k, float2 v) { inner[k] = gn_inner_of(v, __ldg(stats + k).y, g.inv_m); });
-  if (g.cluster > 1) cluster_arrive();
+  if (g.cluster > 1) cluster_arrive_relaxed();
   __syncthreads();
   if (w.on && dx != nullptr) {
     GnInner s;

@@ -348,9 +348,9 @@ int spio_layernorm_2d_bwd(void* dx, float* dweight, float* dbias, const void* dy
  *   bwd: dx (NULL: not wanted), dweight and dbias (fp32 [c], NULL: not wanted) from dy, stats and
  *        either x or, if codes and exponents are given, the values they stand for; sums are added in
  *        a fixed order.  bias is needed where the activation has a slope.
- * Tensors are 16-byte aligned, codes and stats 8-byte, exponents 4-byte.  scratch is device memory of at least
- * the size that the call before it gives for the descriptor on the current device (which may be 0: NULL will do),
- * 16-byte aligned; its contents do not matter. */
+ * Tensors are 16-byte aligned (y and dx of fp32 32-byte), codes and stats 8-byte, exponents 4-byte.
+ * scratch is device memory of at least the size that the call before it gives for the descriptor on the
+ * current device (which may be 0: NULL will do), 16-byte aligned; its contents do not matter. */
 enum { SPIO_TYPE_F16 = 0, SPIO_TYPE_BF16 = 1, SPIO_TYPE_F32 = 2 };
 enum { SPIO_ACT_NONE = 0, SPIO_ACT_RELU = 1, SPIO_ACT_SILU = 2, SPIO_ACT_GELU = 3 };
 typedef struct spio_groupnorm_2d_desc {
@@ -376,7 +376,7 @@ int spio_groupnorm_2d_bwd(void* dx, float* dweight, float* dbias, const void* dy
  * which the block's largest magnitude rounds to at most 127; codes are rounded half to even, and stop
  * at 63 where the value would leave the range of the tensor's type.  A block that holds an infinity or
  * a NaN gets the exponent 255 and is restored as NaN.  codes has 8 bytes a block and is 8-byte
- * aligned, exponents one byte a block, x is 16-byte aligned; blocks may be 0. */
+ * aligned, exponents one byte a block, x is 16-byte aligned (restored fp32 32-byte); blocks may be 0. */
 int spio_checkpoint8_pack(void* codes, void* exponents, const void* x, long long blocks, int type, void* stream);
 int spio_checkpoint8_unpack(void* x, const void* codes, const void* exponents, long long blocks, int type,
                             void* stream);

@@ -327,10 +327,12 @@ int launch(const void* func, unsigned grid, int threads, int smem, int cluster, 
   return 0;
 }
 
-int check_pointers(const void* a, const void* b, const void* c, const void* codes, const void* exponents,
-                   const void* stats) {
-  if (((reinterpret_cast<size_t>(a) | reinterpret_cast<size_t>(b) | reinterpret_cast<size_t>(c)) & 15u) != 0)
+int check_pointers(const spio_groupnorm_2d_desc* d, const void* out, const void* a, const void* b, const void* codes,
+                   const void* exponents, const void* stats) {
+  if (((reinterpret_cast<size_t>(out) | reinterpret_cast<size_t>(a) | reinterpret_cast<size_t>(b)) & 15u) != 0)
     return jit_fail("tensor pointers must be 16-byte aligned");
+  if (d->type == 2 && (reinterpret_cast<size_t>(out) & 31u) != 0)
+    return jit_fail("fp32 tensors that are written must be 32-byte aligned");
   if ((codes == nullptr) != (exponents == nullptr)) return jit_fail("codes and exponents go together");
   if (((reinterpret_cast<size_t>(codes) | reinterpret_cast<size_t>(stats)) & 7u) != 0)
     return jit_fail("codes and stats must be 8-byte aligned");
@@ -359,7 +361,7 @@ int spio_groupnorm_2d_fwd(void* y, float* stats, void* codes, void* exponents, c
   if (check_desc(desc)) return 1;
   if (desc->n == 0 || desc->pixels == 0) return 0;
   if (y == nullptr || x == nullptr) return jit_fail("NULL tensor pointer");
-  if (check_pointers(y, x, scratch, codes, exponents, stats)) return 1;
+  if (check_pointers(desc, y, x, scratch, codes, exponents, stats)) return 1;
   Device dev;
   Plan p;
   const int coded = codes != nullptr;
@@ -399,7 +401,7 @@ int spio_groupnorm_2d_bwd(void* dx, float* dweight, float* dbias, const void* dy
     return 0;
   }
   if (dy == nullptr || stats == nullptr || (x == nullptr && codes == nullptr)) return jit_fail("NULL tensor pointer");
-  if (check_pointers(dx, dy, codes == nullptr ? x : nullptr, codes, exponents, stats)) return 1;
+  if (check_pointers(desc, dx, dy, codes == nullptr ? x : nullptr, codes, exponents, stats)) return 1;
   if ((reinterpret_cast<size_t>(scratch) & 15u) != 0) return jit_fail("scratch must be 16-byte aligned");
   const int coded = codes != nullptr;
   Device dev;

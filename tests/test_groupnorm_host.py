@@ -49,6 +49,11 @@ def test_library_refuses_pointers():
         assert bwd(*args, None, None, desc(), 16, 1 << 20, None) != 0 and message in _clib.last_error(), args
     assert bwd(16, None, None, 16, 16, None, None, 16, None, None, desc(), 8, 1 << 20, None) != 0
     assert "16-byte" in _clib.last_error()
+    # fp32 pieces of 32 bytes are written at once
+    assert fwd(16, None, None, None, 16, None, None, desc(type=2), 16, 1 << 20, None) != 0 and "32-byte" in _clib.last_error()
+    assert bwd(16, None, None, 16, 16, None, None, 16, None, None, desc(type=2), 16, 1 << 20, None) != 0
+    assert "32-byte" in _clib.last_error()
+    assert lib.spio_checkpoint8_unpack(16, 16, 16, 1, 2, None) != 0 and "32-byte" in _clib.last_error()
     # nothing to do is no error: an empty batch, no gradient asked for
     assert fwd(None, None, None, None, None, None, None, desc(n=0), None, 0, None) == 0
     assert bwd(None, None, None, None, None, None, None, None, None, None, desc(), None, 0, None) == 0

@@ -792,8 +792,14 @@ __device__ __forceinline__ void gn_cluster_sums(const GnGeom& g, const GnWork& w
 // ---------------------------------------------------------------- two launches
 //
 // For a few large images: any number of CTAs works on an image, the sums go through memory (one value for each
-// cluster), and the second launch reads the input again.  It may ask for it before the first has ended (its inputs were there before that began) and
-// goes through the data backwards, so that it finds in L2 what the first launch read last.
+// cluster), and the second launch reads the input again.  It may ask for it before the first has ended (its inputs
+// were there before that began) and goes through the data backwards, so that it finds in L2 what the first launch
+// read last.
+//
+// Measured at 1 x 128 x 512 x 512 bf16 with SiLU and 32 groups: 43.9 us for both launches forward (3060 GB/s counting
+// x and y once, where the device copies 6520; under the profiler 19 us for the sums and 25 for the rest), one launch of
+// clusters of 16 72 us.  The first launch waits for memory; the second issues in 42 % of its cycles, keeps the special
+// functions busy for 52 % of them and waits for L2 otherwise.
 
 // part_stats[(image * groups + group) * clusters + cluster] = {mean, centred squares} over the cluster's pixels
 template <class T>
@@ -994,8 +1000,17 @@ groupnorm_2d_bwd_apply_kernel(T* __restrict__ dx, const float2* __restrict__ par
 //
 // The parts of a slab are the CTAs of a cluster (1 to 16) and the sums cross CTAs through distributed shared
 // memory, so one launch does both passes and the second one finds its data close by: it goes through the pieces
-// backwards, those that are still in the ring first (all of them, where a part fits), the others again from L2,
-// which holds what the resident CTAs work on many times over.
+// backwards, those that are still in the ring first (all of them, where a part fits), the others again from L2.
+//
+// Measured at 256 x 64 x 56 x 56 fp16 with SiLU and 8 groups: 49.6 us forward (4140 GB/s counting x and y once, 64 % of
+// what a copy reaches), 85.4 us backward with the sum of the parts (3610 GB/s, 55 %); 28.4 and 41.5 us at
+// 128 x 192 x 28 x 28 with 8-bit codes.  Nothing is used up: forward 51 % of the issue slots and 51 % of the special
+// functions (two a value), backward 49 % and 59 % (four a value).  The CTAs of an SM begin together, so that they load and
+// compute in turn more than at a time.  What did not help: a CTA that goes on to the next image and requests it
+// during its second pass (the bookkeeping of an image came back as waiting), five CTAs of 96 registers instead of four of
+// 128 (88.6 us backward), smaller parts (the second pass of the backward kernel finds 130 of 205 MB no longer in L2; with
+// parts of a quarter of that size it takes 88.3 us, because they pay the reductions more often), one reciprocal for
+// two values, keeping the first pass's gradients in shared memory.
 
 template <class T, int ACT, bool CODES>
 __global__ void __launch_bounds__(kGnThreads, 768 / kGnThreads)

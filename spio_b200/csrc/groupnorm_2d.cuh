@@ -16,6 +16,7 @@
 #include <cuda_runtime.h>
 
 #include "checkpoint8.cuh"
+#include "cluster.cuh"
 #include "groupnorm_2d.h"
 
 #ifndef GN_THREADS
@@ -729,20 +730,6 @@ struct GnBackRing {
 };
 
 // ---------------------------------------------------------------- sums over a cluster
-
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
-// (by threads that have nothing to show, only read)
-__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
-
-// *p of the CTA `rank` of the cluster
-__device__ __forceinline__ float2 cluster_load(const float2* p, int rank) {
-  u32 at;
-  float2 v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
-  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
-  return v;
-}
 
 // Calls body(group, rank, live) with the CTAs of the cluster in neighbouring lanes for each group: all lanes of a warp
 // together, `live` where there is such a group.

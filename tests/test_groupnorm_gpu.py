@@ -202,6 +202,13 @@ def test_sizes_where_only_the_checkpoint_takes_two_launches(shape, groups, act, 
         check_all(shape, groups, dtype, act, checkpoint8, seed=18)
 
 
+@pytest.mark.parametrize("shape,groups", [((1500, 24, 2, 1), 3), ((4097, 8, 1, 3), 1), ((2049, 64, 3, 3), 8)], ids=str)
+def test_many_small_images(shape, groups):
+    """Gradients of weight and bias that are summed over the images by the CTAs of a cluster."""
+    check_all(shape, groups, torch.float16, "relu", seed=21)
+    check_all(shape, groups, torch.bfloat16, "gelu", True, seed=22)
+
+
 def test_forward_mode_derivatives_are_refused():
     x, dy, w, b = make((2, 16, 4, 4), torch.float32, seed=19)
     stats = groupnorm_2d_op(x, w, b, 4, 1e-5, "none", False)[1]

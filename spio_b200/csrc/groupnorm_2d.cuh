@@ -783,7 +783,7 @@ __device__ __forceinline__ void gn_cluster_sums(const GnGeom& g, const GnWork& w
 // were there before that began) and goes through the data backwards, so that it finds in L2 what the first launch
 // read last.
 //
-// Measured at 1 x 128 x 512 x 512 bf16 with SiLU and 32 groups: 43.9 us for both launches forward (3060 GB/s counting
+// Measured at 1 x 128 x 512 x 512 bf16 with SiLU and 32 groups: 42.8 us for both launches forward (3140 GB/s counting
 // x and y once, where the device copies 6520; under the profiler 19 us for the sums and 25 for the rest), one launch of
 // clusters of 16 72 us.  The first launch waits for memory; the second issues in 42 % of its cycles, keeps the special
 // functions busy for 52 % of them and waits for L2 otherwise.
@@ -826,43 +826,57 @@ groupnorm_2d_stats_kernel(float2* __restrict__ part_stats, const T* __restrict__
 // Pixels of an image before part i.
 __device__ __forceinline__ int gn_part_begin(const GnGeom& g, int i) { return i * g.part_px + min(i, g.part_rest); }
 
-// body(value, cluster) for this lane's share of the clusters' values of a group.  Eight loads at a time: every CTA of
-// the second launch does this before anything else, and one load after the other took it 17 us for the 222
-// clusters of 1 x 128 x 512 x 512.
-template <class Body>
-__device__ __forceinline__ void gn_each_cluster(const float2* __restrict__ values, int clusters, Body body) {
+// body(which, value, cluster) for this lane's share of the clusters' values of G groups, kGnWarps apart from group k on
+// (zeros behind the last cluster and for groups that there are not).  G * 8 loads at a time: every CTA of the second launch does this before anything else,
+// and one load after the other took it 17 us for the 222 clusters of 1 x 128 x 512 x 512.
+constexpr int kGnWarps = kGnThreads / 32;
+template <int G, class Body>
+__device__ __forceinline__ void gn_each_cluster(const float2* __restrict__ values, int clusters, int k, int groups,
+                                                Body body) {
   const int lane = threadIdx.x & 31;
   for (int base = 0; base < clusters; base += 256) {
-    float2 v[8];
+    float2 v[G][8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int i = base + j * 32 + lane;
-      v[j] = i < clusters ? __ldcg(values + i) : make_float2(0.f, 0.f);
+    for (int h = 0; h < G; ++h) {
+      const float2* from = values + (long long)(k + h * kGnWarps) * clusters;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int i = base + j * 32 + lane;
+        v[h][j] = k + h * kGnWarps < groups && i < clusters ? __ldcg(from + i) : make_float2(0.f, 0.f);
+      }
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (base + j * 32 + lane < clusters) body(v[j], base + j * 32 + lane);
+    for (int h = 0; h < G; ++h) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) body(h, v[h][j], base + j * 32 + lane);
+    }
   }
 }
 
 // Mean and rstd of the slab's groups from the clusters' values, into stat[]; all threads, synchronised.
 __device__ __forceinline__ void gn_merge_parts(float2* stat, const GnGeom& g, const GnWork& w,
                                                const float2* __restrict__ part_stats) {
-  const long long first_group = gn_first_group(g, w);
+  constexpr int G = 2;
   const int clusters = g.parts >> g.log_cluster;
-  for (int k = threadIdx.x >> 5; k < w.groups; k += kGnThreads / 32) {
-    const float2* ps = part_stats + (first_group + k) * clusters;
-    const float m0 = __ldcg(ps).x;  // (differences to one of the means: little cancels)
-    float s = 0.f, q = 0.f;
-    gn_each_cluster(ps, clusters, [&](float2 v, int i) {
-      const float n = (float)(gn_part_begin(g, (i + 1) << g.log_cluster) - gn_part_begin(g, i << g.log_cluster));
-      const float d = v.x - m0;
-      s = fmaf(n, d, s);
-      q += fmaf(n * (float)g.cpg * d, d, v.y);
+  const float2* first = part_stats + gn_first_group(g, w) * clusters;
+  for (int k = threadIdx.x >> 5; k < w.groups; k += G * kGnWarps) {
+    float m0[G], s[G] = {}, q[G] = {};
+    gn_each_cluster<G>(first, clusters, k, w.groups, [&](int h, float2 v, int i) {
+      if (i == (int)(threadIdx.x & 31)) m0[h] = __shfl_sync(0xffffffffu, v.x, 0);  // (differences to the first mean: little cancels)
+      const float n = i < clusters
+                          ? (float)(gn_part_begin(g, (i + 1) << g.log_cluster) - gn_part_begin(g, i << g.log_cluster))
+                          : 0.f;
+      const float d = v.x - m0[h];
+      s[h] = fmaf(n, d, s[h]);
+      q[h] += fmaf(n * (float)g.cpg * d, d, v.y);
     });
-    s = sum_lanes(s, 5), q = sum_lanes(q, 5);
-    const float d = s * g.inv_pixels, m2 = not_below_zero(fmaf(-s * (float)g.cpg, d, q));
-    if ((threadIdx.x & 31) == 0) stat[k] = make_float2(m0 + d, rsqrtf(fmaf(m2, g.inv_m, g.eps)));
+#pragma unroll
+    for (int h = 0; h < G; ++h) {
+      const float sum = sum_lanes(s[h], 5), square = sum_lanes(q[h], 5);
+      const float d = sum * g.inv_pixels, m2 = not_below_zero(fmaf(-sum * (float)g.cpg, d, square));
+      if ((threadIdx.x & 31) == 0 && k + h * kGnWarps < w.groups)
+        stat[k + h * kGnWarps] = make_float2(m0[h] + d, rsqrtf(fmaf(m2, g.inv_m, g.eps)));
+    }
   }
   __syncthreads();
 }
@@ -965,12 +979,18 @@ groupnorm_2d_bwd_apply_kernel(T* __restrict__ dx, const float2* __restrict__ par
   grid_dependency_launch_dependents();
   const long long first_group = gn_first_group(g, w);
   stats += first_group;
+  constexpr int G = 4;
   const int clusters = g.parts >> g.log_cluster;
-  for (int k = threadIdx.x >> 5; k < w.groups; k += kGnThreads / 32) {
-    float s = 0.f, q = 0.f;
-    gn_each_cluster(part_group + (first_group + k) * clusters, clusters, [&](float2 v, int) { s += v.x, q += v.y; });
-    s = sum_lanes(s, 5), q = sum_lanes(q, 5);
-    if ((threadIdx.x & 31) == 0) inner[k] = gn_inner_of(make_float2(s, q), __ldg(stats + k).y, g.inv_m);
+  for (int k = threadIdx.x >> 5; k < w.groups; k += G * kGnWarps) {
+    float s[G] = {}, q[G] = {};
+    gn_each_cluster<G>(part_group + first_group * clusters, clusters, k, w.groups,
+                       [&](int h, float2 v, int) { s[h] += v.x, q[h] += v.y; });
+#pragma unroll
+    for (int h = 0; h < G; ++h) {
+      const float a = sum_lanes(s[h], 5), b = sum_lanes(q[h], 5);
+      if ((threadIdx.x & 31) == 0 && k + h * kGnWarps < w.groups)
+        inner[k + h * kGnWarps] = gn_inner_of(make_float2(a, b), __ldg(stats + k + h * kGnWarps).y, g.inv_m);
+    }
   }
   __syncthreads();
   if (!w.on) return;

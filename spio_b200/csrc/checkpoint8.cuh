@@ -33,11 +33,13 @@ struct Piece {
   uint4 u[W];
 };
 
+// (The kernels start while the one before them may still be writing what they read, and wait for it: so these are
+// loads that stay behind the wait, and that do not take the data for constant during the kernel.)
 template <class T>
 __device__ __forceinline__ Piece<T> load_piece(const T* p) {
   Piece<T> v;
 #pragma unroll
-  for (int i = 0; i < Piece<T>::W; ++i) v.u[i] = reinterpret_cast<const uint4*>(p)[i];
+  for (int i = 0; i < Piece<T>::W; ++i) v.u[i] = __ldcg(reinterpret_cast<const uint4*>(p) + i);
   return v;
 }
 

@@ -354,8 +354,8 @@ __device__ __forceinline__ GnAffine gn_affine(const GnWork& w, const float* __re
   const int channel = (w.first + w.p) * 8;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    a.weight.p[i] = weight != nullptr ? pair(__ldg(weight + channel + 2 * i), __ldg(weight + channel + 2 * i + 1)) : pair(1.f);
-    a.bias.p[i] = bias != nullptr ? pair(__ldg(bias + channel + 2 * i), __ldg(bias + channel + 2 * i + 1)) : pair(0.f);
+    a.weight.p[i] = weight != nullptr ? pair(__ldca(weight + channel + 2 * i), __ldca(weight + channel + 2 * i + 1)) : pair(1.f);
+    a.bias.p[i] = bias != nullptr ? pair(__ldca(bias + channel + 2 * i), __ldca(bias + channel + 2 * i + 1)) : pair(0.f);
   }
   return a;
 }
@@ -476,7 +476,7 @@ __device__ __forceinline__ void gn_back_groups(const GnGeom& g, const GnWork& w,
       if (weight != nullptr) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float f = __ldg(weight + (w.first + w.p) * 8 + i);
+          const float f = __ldca(weight + (w.first + w.p) * 8 + i);
           a[i] *= f, b[i] *= f;
         }
       }
@@ -494,13 +494,13 @@ __device__ __forceinline__ void gn_back_groups(const GnGeom& g, const GnWork& w,
         });
       } else {
         gn_run(g, w, k, lane, [&](int at, int ch, int) {
-          const float f = weight != nullptr ? __ldg(weight + w.first * 8 + k * g.cpg + ch) : 1.f;
+          const float f = weight != nullptr ? __ldca(weight + w.first * 8 + k * g.cpg + ch) : 1.f;
           s = fmaf(f, red.a[at], s), q = fmaf(f, red.b[at], q);
         });
       }
     }
     s = sum_lanes(s, g.lanes), q = sum_lanes(q, g.lanes);
-    if (live && lane == 0) put(k, make_float2(s * __ldg(stats + k).y, q));
+    if (live && lane == 0) put(k, make_float2(s * __ldca(stats + k).y, q));
   });
 }
 
@@ -520,7 +520,7 @@ __device__ __forceinline__ void gn_back_channels(const GnGeom& g, const GnWork& 
       for (int r = lane; r < w.rows; r += lanes) s += from[r * row];
     }
     s = sum_lanes(s, g.column_lanes);
-    if (live && lane == 0) out[(second ? g.c : 0) + w.first * 8 + ch] = second ? s : s * __ldg(stats + gn_group(g, ch)).y;
+    if (live && lane == 0) out[(second ? g.c : 0) + w.first * 8 + ch] = second ? s : s * __ldca(stats + gn_group(g, ch)).y;
   }
 }
 
@@ -938,7 +938,7 @@ groupnorm_2d_bwd_sums_kernel(float* __restrict__ part_channel, float2* __restric
   const long long first_group = gn_first_group(g, w);
   stats += first_group;
   GnChannels c;
-  if (w.on) gn_channels(c, g, w, gn_affine(w, weight, bias), [&](int k) { return __ldg(stats + k); });
+  if (w.on) gn_channels(c, g, w, gn_affine(w, weight, bias), [&](int k) { return __ldca(stats + k); });
   GnBackSums t;
   t.clear();
   gn_forwards<B>(count, first, step, issue,
@@ -989,13 +989,13 @@ groupnorm_2d_bwd_apply_kernel(T* __restrict__ dx, const float2* __restrict__ par
     for (int h = 0; h < G; ++h) {
       const float a = sum_lanes(s[h], 5), b = sum_lanes(q[h], 5);
       if ((threadIdx.x & 31) == 0 && k + h * kGnWarps < w.groups)
-        inner[k + h * kGnWarps] = gn_inner_of(make_float2(a, b), __ldg(stats + k + h * kGnWarps).y, g.inv_m);
+        inner[k + h * kGnWarps] = gn_inner_of(make_float2(a, b), __ldca(stats + k + h * kGnWarps).y, g.inv_m);
     }
   }
   __syncthreads();
   if (!w.on) return;
   GnChannels c;
-  gn_channels(c, g, w, gn_affine(w, weight, bias), [&](int k) { return __ldg(stats + k); });
+  gn_channels(c, g, w, gn_affine(w, weight, bias), [&](int k) { return __ldca(stats + k); });
   GnInner s;
   gn_inner(s, g, w, [&](int k) { return inner[k]; });
   gn_forwards<B>(count, first, step, issue, [&](int slot, u32 at) {
@@ -1092,7 +1092,7 @@ groupnorm_2d_bwd_kernel(T* __restrict__ dx, float* __restrict__ part_channel, co
   gn_request<B>(count, first, step, issue);
   stats += gn_first_group(g, w);
   GnChannels c;
-  if (w.on) gn_channels(c, g, w, gn_affine(w, weight, bias), [&](int k) { return __ldg(stats + k); });
+  if (w.on) gn_channels(c, g, w, gn_affine(w, weight, bias), [&](int k) { return __ldca(stats + k); });
   GnBackSums t;
   t.clear();
   gn_forwards<B>(count, first, step, issue,
@@ -1102,7 +1102,7 @@ groupnorm_2d_bwd_kernel(T* __restrict__ dx, float* __restrict__ part_channel, co
   if (part_channel != nullptr) gn_back_channels(g, w, stats, red, part_channel + (w.image * g.parts + w.part) * 2 * g.c);
   if (g.cluster > 1) cluster_wait();
   else __syncthreads();
-  gn_cluster_sums(g, w, own, [&](int k, float2 v) { inner[k] = gn_inner_of(v, __ldg(stats + k).y, g.inv_m); });
+  gn_cluster_sums(g, w, own, [&](int k, float2 v) { inner[k] = gn_inner_of(v, __ldca(stats + k).y, g.inv_m); });
   if (g.cluster > 1) cluster_arrive_relaxed();
   __syncthreads();
   if (w.on && dx != nullptr) {

@@ -100,7 +100,7 @@ def build_torch_lib(force: bool = False, verbose: bool = False) -> Path:
           f"-I{root / 'include'}", f"-I{root / 'include' / 'torch' / 'csrc' / 'api' / 'include'}",
           f"-I{cuda / 'include'}", str(TORCH_SOURCE), "-o", str(TORCH_LIB_PATH),
           f"-L{LIB_DIR}", "-lspio_b200", "-Wl,-rpath,$ORIGIN",
-          f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch"], verbose)
+          f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch"], verbose)
     return TORCH_LIB_PATH
 
 

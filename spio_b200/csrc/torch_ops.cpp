@@ -6,6 +6,7 @@
 // The device work is that of the C ABI (include/spio_b200.h), on torch's current stream.
 #include <ATen/ATen.h>
 #include <ATen/autocast_mode.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -33,11 +34,12 @@ int type_code(at::ScalarType t) {
   }
 }
 
+constexpr int kActivations = 4;
+constexpr c10::string_view kActivationNames[kActivations] = {"none", "relu", "silu", "gelu"};  // by SPIO_ACT_*
+
 int activation_code(c10::string_view name) {
-  if (name == "none") return SPIO_ACT_NONE;
-  if (name == "relu") return SPIO_ACT_RELU;
-  if (name == "silu") return SPIO_ACT_SILU;
-  if (name == "gelu") return SPIO_ACT_GELU;
+  for (int i = 0; i < kActivations; ++i)
+    if (name == kActivationNames[i]) return i;
   TORCH_CHECK_VALUE(false, "activation must be one of none, relu, silu, gelu, got ", std::string(name));
 }
 
@@ -57,13 +59,14 @@ Tensor kernel_layout(const Tensor& t) {
   return c.clone(at::MemoryFormat::ChannelsLast);
 }
 
+// Allocated without the dispatcher: these calls are below it, and a backward pass allocates four tensors.
+Tensor empty(at::IntArrayRef size, const Tensor& like, at::ScalarType type, at::MemoryFormat format = at::MemoryFormat::Contiguous) {
+  return Tensor(at::detail::empty_cuda(size, type, like.device(), format));
+}
 Tensor empty_image(at::IntArrayRef size, const Tensor& like, at::ScalarType type) {
-  return at::empty(size, like.options().dtype(type).memory_format(at::MemoryFormat::ChannelsLast));
+  return empty(size, like, type, at::MemoryFormat::ChannelsLast);
 }
-
-Tensor empty_vector(int64_t n, const Tensor& like, at::ScalarType type) {
-  return at::empty({n}, like.options().dtype(type).memory_format(at::MemoryFormat::Contiguous));
-}
+Tensor empty_vector(int64_t n, const Tensor& like, at::ScalarType type) { return empty({n}, like, type); }
 
 void* pointer(const Tensor& t) { return t.defined() && t.numel() > 0 ? t.data_ptr() : nullptr; }
 float* floats(const Tensor& t) { return static_cast<float*>(pointer(t)); }
@@ -143,7 +146,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> forward(const Tensor& x_, const OptTe
   const Tensor x = kernel_layout(x_), weight = vector_of(weight_), bias = vector_of(bias_);
   const Tensor y = empty_image(x.sizes(), x, x.scalar_type());
   Tensor stats, codes, exponents;
-  if (want_stats) stats = at::empty({x.size(0), num_groups, 2}, x.options().dtype(at::kFloat).memory_format(at::MemoryFormat::Contiguous));
+  if (want_stats) stats = empty({x.size(0), num_groups, 2}, x, at::kFloat);
   if (want_codes) std::tie(codes, exponents) = empty_codes(x);
   const size_t bytes = spio_groupnorm_2d_fwd_scratch_bytes(&desc);
   const Tensor scratch = scratch_of(bytes, x);
@@ -242,8 +245,7 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
       ctx->save_for_backward({Tensor(), codes, exponents, stats, tensor_of(weight), tensor_of(bias)});
     else
       ctx->save_for_backward({x, Tensor(), Tensor(), stats, tensor_of(weight), tensor_of(bias)});
-    ctx->saved_data["num_groups"] = num_groups;
-    ctx->saved_data["activation"] = std::move(activation);
+    ctx->saved_data["call"] = num_groups * kActivations + activation_code(activation);
     return y;
   }
   static variable_list backward(torch::autograd::AutogradContext* ctx, variable_list grads) {
@@ -256,10 +258,12 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
     const bool want_weight = saved[4].defined() && ctx->needs_input_grad(edge++);
     const bool want_bias = saved[5].defined() && ctx->needs_input_grad(edge++);
     const bool want[3] = {want_x, want_weight, want_bias};
+    const int64_t call = ctx->saved_data["call"].toInt();
+    std::optional<at::AutoDispatchBelowADInplaceOrView> below;  // (with grad mode on, the operator refuses what it has to)
+    if (!at::GradMode::is_enabled()) below.emplace();
     auto [dx, dw, db] = backward_op().call(
         grads[0], optional_of(saved[0]), optional_of(saved[1]), optional_of(saved[2]), saved[3], optional_of(saved[4]),
-        optional_of(saved[5]), ctx->saved_data["num_groups"].toInt(), ctx->saved_data["activation"].toStringRef(), want[0],
-        want[1], want[2]);
+        optional_of(saved[5]), call / kActivations, kActivationNames[call % kActivations], want[0], want[1], want[2]);
     if (want[0]) result[0] = dx;
     if (want[1]) result[1] = dw;
     if (want[2]) result[2] = db;
@@ -384,9 +388,8 @@ struct ConvCheckpoint8 : torch::autograd::Function<ConvCheckpoint8> {
     const Tensor y = conv_forward(c, x, weight, bias);
     auto [codes, exponents] = checkpoint8_pack(x);
     ctx->save_for_backward({codes, exponents, weight, tensor_of(bias)});
-    ctx->saved_data["pad_y"] = pad_y;
-    ctx->saved_data["pad_x"] = pad_x;
-    ctx->saved_data["tunes"] = std::move(tunes);
+    tunes.push_back(pad_y), tunes.push_back(pad_x);
+    ctx->saved_data["call"] = std::move(tunes);
     return y;
   }
   static variable_list backward(torch::autograd::AutogradContext* ctx, variable_list grads) {
@@ -401,8 +404,9 @@ struct ConvCheckpoint8 : torch::autograd::Function<ConvCheckpoint8> {
     const c10::cuda::CUDAGuard guard(codes.device());
     // the sizes of the input are those of its codes; its values are read for the weight gradient alone
     const Tensor x = want_w ? checkpoint8_unpack(codes, exponents, at::kHalf) : empty_image(codes.sizes(), codes, at::kHalf);
-    const Conv c = conv_of(x, weight, optional_of(saved[3]), ctx->saved_data["pad_y"].toInt(),
-                           ctx->saved_data["pad_x"].toInt(), ctx->saved_data["tunes"].toIntVector());
+    const std::vector<int64_t> call = ctx->saved_data["call"].toIntVector();  // tunes, padding
+    const Conv c = conv_of(x, weight, optional_of(saved[3]), call[call.size() - 2], call.back(),
+                           at::IntArrayRef(call).slice(0, call.size() - 2));
     const Tensor dy = kernel_layout(grads[0]), w = kernel_layout(weight);
     Tensor dx, dw, db;
     if (want_x) dx = empty_image(x.sizes(), x, at::kHalf);

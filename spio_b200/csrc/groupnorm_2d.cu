@@ -216,11 +216,11 @@ void set_ring(Plan* p, int type, int bytes, bool backward) {
 // Which launch to make.  The alternatives differ in the width of a slab, the CTAs of a cluster and their threads, or
 // take two launches; none is best for all sizes.  Narrow slabs and large clusters give CTAs enough to fill the
 // device, wide slabs whole DRAM sectors, few CTAs little bookkeeping, two launches any number of CTAs for one
-// image.  The costs are estimates in cycles with constants fitted to 2500 measured launches of 60 sizes (all types,
-// activations and directions; 0.01 to 51 million values): the choice takes 4 % longer than the best of each size on
-// average, 31 % at worst (8 us instead of 11).
+// image.  The costs are estimates in cycles with constants fitted to 14000 measured launches of 300 sizes (all types,
+// activations and directions; 0.2 to 64 million values): the choice takes 3 % longer than the best of each size on
+// average, 42 % at worst (28 us instead of 19).
 struct Work {
-  double values, piece, read, written;  // instructions a warp spends on a piece in both passes; bytes
+  double values, piece, piece_bytes, read, written;  // piece: instructions a warp spends on it in both passes
 };
 
 Work work_of(const spio_groupnorm_2d_desc* d, bool backward, bool coded) {
@@ -229,6 +229,7 @@ Work work_of(const spio_groupnorm_2d_desc* d, bool backward, bool coded) {
   const double size = d->type == 2 ? 4 : 2;
   Work w;
   w.values = (double)d->n * d->pixels * d->c;
+  w.piece_bytes = 8 * size;
   w.piece = (backward ? 110 + 85 * act + (coded ? 20 : 0) : 72 + 28 * act + (coded ? 25 : 0)) + (d->type == 2 ? 15 : 0);
   w.read = w.values * (backward ? size + (coded ? 1.125 : size) : size);
   w.written = w.values * (size + (coded && !backward ? 1.125 : 0));
@@ -244,22 +245,31 @@ double cost_of_one_launch(const Plan& p, const Work& w, const Device& dev, bool 
   const int on_sm = std::max(1, std::min((backward ? 512 : 768) / p.threads, 228 * 1024 / (p.smem + 1024)));
   const double of_sm = std::ceil(ctas / dev.sms), rounds = std::ceil(of_sm / on_sm);
   const double warps = std::min(of_sm, (double)on_sm) * p.threads / 32;
-  const double instructions = of_sm * p.threads / 32 * ((backward ? 1060 : 640) + pieces * w.piece);
-  const double compute = instructions / std::min(5.75, .248 * warps);
-  const double row = g.sp * 8. * (w.written >= 4 * w.values ? 4 : 2);  // bytes of a pixel
-  const double again = std::max(0., 1. - (double)p.slots / pieces) * w.read * 1.4;  // from L2
-  const double memory = (w.read + w.written + again) / kBytesPerCycle / (row >= 64 ? 1. : row >= 32 ? .71 : .69);
-  const double sync = g.cluster > 1 ? 840 + 550 * g.log_cluster : 0;
+  const double instructions = of_sm * p.threads / 32 * ((backward ? 969 : 645) + (g.fold ? 0 : 195) + pieces * w.piece);
+  const double compute = instructions / std::min(3.9, .358 * warps);
+  const double row = g.sp * w.piece_bytes;
+  const double again = std::max(0., 1. - (double)p.slots / pieces) * w.read * (backward ? .845 : 2.54);  // from L2
+  const double filled = std::min(1., 2.19 * ctas * p.threads / (dev.sms * 256.));  // few threads have little on its way
+  const double memory =
+      (w.read + w.written + again) / kBytesPerCycle / (row >= 64 ? 1. : row >= 32 ? .6 : .36) / filled;
+  const double sync = g.cluster > 1 ? 380 + 587 * g.log_cluster : 0;
   // (the CTAs of an SM start together, and load and compute in turn more than at a time)
-  return .83 * std::max(compute, memory) + 1.17 * std::min(compute, memory) +
-         rounds * ((backward ? 710 : 1800) + sync) + (backward ? 7900 : 4700);
+  return .82 * std::max(compute, memory) + 1.45 * std::min(compute, memory) +
+         rounds * ((backward ? 1620 : 1270) + sync) + (backward ? 6890 : 3490);
 }
 
-double cost_of_two_launches(const Work& w, const Device& dev, bool backward) {
-  const double compute = w.values / 8 / 32 / dev.sms * (w.piece + 10) / 2.34;
-  const double far = std::min(1., std::max(0., (w.read - 4e7) / 8e7));  // share of the second reading that L2 has lost
-  const double memory = (w.read * (1. + .87 + .13 * far) + w.written) / kBytesPerCycle;
-  return 1.17 * std::max(compute, memory) + .36 * std::min(compute, memory) + (backward ? 20300 : 15400);
+double cost_of_two_launches(const Plan& p, const Work& w, const Device& dev, bool backward) {
+  const GnGeom& g = p.g;
+  if (g.parts == 1) return std::numeric_limits<double>::infinity();  // the same CTAs do it in one launch
+  const double of_sm = std::ceil((double)g.images * g.slabs * g.parts / dev.sms);
+  const int pieces = cdiv(cdiv(g.pixels, g.parts), p.threads / g.sp);
+  const double compute = of_sm * p.threads / 32 * (458 + pieces * (w.piece + 10)) / 2.28;
+  // pixels' segments that begin and end inside a cache line cost where L2 does not hold them until the rest is wanted
+  const double row = g.sp * w.piece_bytes, beyond = std::min(1., std::max(0., (w.read + w.written - 5e7) / 1e8));
+  const double torn = g.slabs > 1 && (g.sp * (int)w.piece_bytes) % 128 != 0 ? 14.5 / row * beyond : 0.;
+  const double memory = (1.25 * w.read + w.written) * (1. + torn) / kBytesPerCycle;
+  const double merges = cdiv(g.slab_groups, 8 * (backward ? 4 : 2)) * cdiv(g.parts / g.cluster, 256);
+  return .9 * std::max(compute, memory) + .73 * std::min(compute, memory) + 1020 * merges + (backward ? 14000 : 10100);
 }
 
 int choose_plan(const spio_groupnorm_2d_desc* d, const Device& dev, bool backward, bool coded, Plan* best) {
@@ -279,16 +289,20 @@ int choose_plan(const spio_groupnorm_2d_desc* d, const Device& dev, bool backwar
   const int bytes = backward ? piece + (coded ? 12 : piece) : piece;  // of a ring's slot
   const Work w = work_of(d, backward, coded);
 
-  // two launches: slabs of 64 pieces (1 KB of a pixel) where a group allows it, as many CTAs as fit on the device, but
-  // four pixels a thread at least
+  // two launches: as many CTAs as fit on the device, but four pixels a thread at least; slabs of at most 64 pieces (1 KB of
+  // a pixel) where a group allows it, and narrower ones, which leave each CTA of the second launch less to merge
+  double least = std::numeric_limits<double>::infinity();
   p.one_launch = false;
   p.threads = kGnWide;
-  set_slabs(&g, unit, std::max(1, 64 / unit));
-  set_many_parts(&g, dev, backward);
-  set_ring(&p, d->type, bytes, backward);
-  *best = p;
-  // (one part: the same CTAs do it in one launch)
-  double least = g.parts > 1 ? cost_of_two_launches(w, dev, backward) : std::numeric_limits<double>::infinity();
+  for (int most = 64, sp = 0; most >= 8; most /= 2) {
+    set_slabs(&g, unit, std::max(1, most / unit));
+    if (g.sp == sp) continue;
+    sp = g.sp;
+    set_many_parts(&g, dev, backward);
+    set_ring(&p, d->type, bytes, backward);
+    const double cost = cost_of_two_launches(p, w, dev, backward);
+    if (cost < least) least = cost, *best = p;
+  }
 
   p.one_launch = true;
   for (int most = std::min(units, std::max(1, 64 / unit)), sp = 0; most >= 1; --most) {
@@ -307,6 +321,7 @@ int choose_plan(const spio_groupnorm_2d_desc* d, const Device& dev, bool backwar
       }
     }
   }
+  if (!(least < std::numeric_limits<double>::infinity())) return jit_fail("GroupNorm2d: no launch fits the device");
   const GnGeom& b = best->g;
   const long long grid = b.images * b.slabs * b.parts;
   if (grid > 0x7fffffffll) return jit_fail("GroupNorm2d: too many images for one launch");

@@ -783,8 +783,8 @@ __device__ __forceinline__ void gn_cluster_sums(const GnGeom& g, const GnWork& w
 // were there before that began) and goes through the data backwards, so that it finds in L2 what the first launch
 // read last.
 //
-// Measured at 1 x 128 x 512 x 512 bf16 with SiLU and 32 groups: 42.8 us for both launches forward (3140 GB/s counting
-// x and y once, where the device copies 6520; under the profiler 19 us for the sums and 25 for the rest), one launch of
+// Measured at 1 x 128 x 512 x 512 bf16 with SiLU and 32 groups: 41.2 us for both launches forward (3260 GB/s counting
+// x and y once, where the device copies 6520; under the profiler 19 us for the sums and 23 for the rest), one launch of
 // clusters of 16 72 us.  The first launch waits for memory; the second issues in 42 % of its cycles, keeps the special
 // functions busy for 52 % of them and waits for L2 otherwise.
 

@@ -202,6 +202,16 @@ def test_sizes_where_only_the_checkpoint_takes_two_launches(shape, groups, act, 
         check_all(shape, groups, dtype, act, checkpoint8, seed=18)
 
 
+@pytest.mark.parametrize("shape,groups,act,dtype", [((1, 160, 140, 170), 32, "silu", torch.float16),
+                                                    ((1, 256, 140, 170), 64, "gelu", torch.bfloat16),
+                                                    ((1, 520, 100, 111), 13, "silu", torch.float16),
+                                                    ((1, 448, 75, 131), 7, "none", torch.float32)], ids=str)
+def test_one_large_image(shape, groups, act, dtype):
+    """(On a B200.)  Two launches with several slabs of channels, the last of them narrower."""
+    for checkpoint8 in (False, True):
+        check_all(shape, groups, dtype, act, checkpoint8, seed=23)
+
+
 @pytest.mark.parametrize("shape,groups", [((1500, 24, 2, 1), 3), ((4097, 8, 1, 3), 1), ((2049, 64, 3, 3), 8)], ids=str)
 def test_many_small_images(shape, groups):
     """Gradients of weight and bias that are summed over the images by the CTAs of a cluster."""

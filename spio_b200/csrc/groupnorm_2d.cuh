@@ -784,9 +784,9 @@ __device__ __forceinline__ void gn_cluster_sums(const GnGeom& g, const GnWork& w
 // read last.
 //
 // Measured at 1 x 128 x 512 x 512 bf16 with SiLU and 32 groups: 41.2 us for both launches forward (3260 GB/s counting
-// x and y once, where the device copies 6520; under the profiler 19 us for the sums and 23 for the rest), one launch of
-// clusters of 16 72 us.  The first launch waits for memory; the second issues in 42 % of its cycles, keeps the special
-// functions busy for 52 % of them and waits for L2 otherwise.
+// x and y once, where the device copies 6520; under the profiler 19 us for the sums and 27 for the rest, which finds
+// nothing in L2 there), one launch of clusters of 16 72 us.  The first launch waits for memory; the second issues in 46 %
+// of its cycles and keeps the special functions busy for 65 % of them.
 
 // part_stats[(image * groups + group) * clusters + cluster] = {mean, centred squares} over the cluster's pixels
 template <class T>
@@ -1015,7 +1015,7 @@ groupnorm_2d_bwd_apply_kernel(T* __restrict__ dx, const float2* __restrict__ par
 // functions (two a value), backward 49 % and 59 % (four a value).  The CTAs of an SM begin together, so that they load and
 // compute in turn more than at a time.  What did not help: a CTA that goes on to the next image and requests it
 // during its second pass (the bookkeeping of an image came back as waiting), five CTAs of 96 registers instead of four of
-// 128 (88.6 us backward), smaller parts (the second pass of the backward kernel finds 130 of 205 MB no longer in L2; with
+// 128 (88.6 us backward), smaller parts (the second pass of the backward kernel finds 120 of 206 MB no longer in L2; with
 // parts of a quarter of that size it takes 88.3 us, because they pay the reductions more often), one reciprocal for
 // two values, keeping the first pass's gradients in shared memory.
 

@@ -6,7 +6,8 @@
 namespace spio_b200 {
 
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
-// (by threads that have nothing to show, only read)
+// For threads that have neither written what another CTA reads nor read another CTA's memory: it orders nothing, so that
+// loads issued before it may still be under way when the other CTAs pass the barrier and leave.
 __device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 

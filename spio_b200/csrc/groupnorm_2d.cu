@@ -76,7 +76,9 @@ groupnorm_2d_bwd_reduce_kernel(float* __restrict__ dweight, float* __restrict__ 
 #pragma unroll
       for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
     }
-    cluster_arrive_relaxed();
+    // (the first has read the others' sums, which are there until it has arrived)
+    if (rank == 0) cluster_arrive();
+    else cluster_arrive_relaxed();
   }
   const int out = block * 32 + warp;
   if (rank == 0 && lane == 0 && out < 2 * c) {
@@ -86,7 +88,7 @@ groupnorm_2d_bwd_reduce_kernel(float* __restrict__ dweight, float* __restrict__ 
       dbias[out - c] = s;
     }
   }
-  if (SPLIT) cluster_wait();  // no CTA leaves while the first reads its sums
+  if (SPLIT) cluster_wait();
 }
 
 struct Plan {

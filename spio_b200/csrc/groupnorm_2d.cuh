@@ -750,6 +750,15 @@ __device__ __forceinline__ void gn_cluster_sync(const GnGeom& g) {
   }
 }
 
+// Arrives for the last time, behind the sums over the cluster: a CTA may leave once all have arrived, and with it the
+// memory that the others read.  So the warps that gn_over_cluster gave something to read release their arrival; the
+// others read nothing and need no order (a release costs a warp some hundred cycles).
+__device__ __forceinline__ void gn_cluster_done(const GnGeom& g, const GnWork& w) {
+  if (g.cluster == 1) return;
+  if ((int)(threadIdx.x & ~31u) >> g.log_cluster < w.groups) cluster_arrive();
+  else cluster_arrive_relaxed();
+}
+
 __device__ __forceinline__ float2 gn_of_rank(const GnGeom& g, const float2* own, int rank) {
   return g.cluster > 1 ? cluster_load(own, rank) : *own;
 }
@@ -1056,8 +1065,8 @@ groupnorm_2d_fwd_kernel(T* __restrict__ y, float2* __restrict__ stats, uint2* __
     stat[k] = st;
     if (stats != nullptr && w.part == 0) stats[gn_first_group(g, w) + k] = st;
   });
-  if (g.cluster > 1) cluster_arrive_relaxed();  // (this CTA has read the others' values; waited for at the end)
   __syncthreads();
+  gn_cluster_done(g, w);  // waited for at the end
   if (w.on) {
     GnChannels c;
     gn_channels(c, g, w, affine, [&](int k) { return stat[k]; });
@@ -1103,8 +1112,8 @@ groupnorm_2d_bwd_kernel(T* __restrict__ dx, float* __restrict__ part_channel, co
   if (g.cluster > 1) cluster_wait();
   else __syncthreads();
   gn_cluster_sums(g, w, own, [&](int k, float2 v) { inner[k] = gn_inner_of(v, __ldca(stats + k).y, g.inv_m); });
-  if (g.cluster > 1) cluster_arrive_relaxed();
   __syncthreads();
+  gn_cluster_done(g, w);
   if (w.on && dx != nullptr) {
     GnInner s;
     gn_inner(s, g, w, [&](int k) { return inner[k]; });

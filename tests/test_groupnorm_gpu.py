@@ -377,3 +377,17 @@ def test_offsets_beyond_32_bits():
     dx, dw, db = groupnorm_2d_backward_op(y, None, codes, exponents, stats, None, None, 8, "none", True, True, True)
     assert bool(dx[-1].isfinite().all()) and not bool(dx[0].any())
     torch.testing.assert_close(db, y[-1].double().sum((1, 2)).float(), rtol=0, atol=CONST * float(y[-1].double().abs().sum((1, 2)).max()))
+
+
+@pytest.mark.parametrize("shape,groups", [((64, 64, 23, 23), 8), ((9, 256, 37, 29), 64), ((7, 24, 61, 53), 3),
+                                          ((2051, 8, 3, 1), 1)], ids=str)
+def test_clusters_one_behind_the_other(shape, groups):
+    """Launches back to back, so that clusters begin where others have just left: their CTAs read each other's sums
+    (groups of the slab fewer and more than a warp can take, parts of unequal size, the sum over many images)."""
+    x, dy, w, b = make(shape, torch.float16, seed=26)
+    check_all(shape, groups, torch.float16, "silu", seed=26)
+    results = []
+    for _ in range(20):
+        y, stats, _, _ = groupnorm_2d_op(x, w, b, groups, 1e-5, "silu", False)
+        results.append((y, stats, *groupnorm_2d_backward_op(dy, x, None, None, stats, w, b, groups, "silu", True, True, True)))
+    assert all(torch.equal(p, q) for r in results[1:] for p, q in zip(r, results[0]))

@@ -369,6 +369,19 @@ int spio_groupnorm_2d_bwd(void* dx, float* dweight, float* dbias, const void* dy
                           const void* exponents, const float* stats, const float* weight, const float* bias,
                           const spio_groupnorm_2d_desc* desc, void* scratch, size_t scratch_bytes, void* stream);
 
+/* The launch of a pass over at least one image and pixel (backward, coded: 0 or 1; coded: it writes or reads the
+ * 8-bit form), for a device with the given SM count and opt-in shared-memory limit; touches no device. */
+typedef struct spio_groupnorm_2d_plan_info {
+  int one_launch;            /* 0: the sums and what follows from them are two launches */
+  int threads, smem_bytes;   /* of a CTA */
+  int slab_pieces, slabs;    /* blocks of 8 channels of a slab, slabs of an image; the last slab may be narrower */
+  int parts, cluster;        /* parts of an image's pixels, of which a cluster has so many */
+  unsigned grid;
+  size_t scratch_bytes;      /* that this pass needs */
+} spio_groupnorm_2d_plan_info;
+int spio_groupnorm_2d_plan_for(const spio_groupnorm_2d_desc* desc, int backward, int coded, int sm_count,
+                               int smem_optin_bytes, spio_groupnorm_2d_plan_info* info);
+
 /* ---- 8-bit form of an activation tensor ----------------------------------------------
  * For activations that are kept for a backward pass: 1.125 bytes a value.  Blocks of 8 consecutive
  * values (one channel group of a pixel in NHWC order) become 8 signed codes and one exponent byte:

@@ -60,6 +60,16 @@ class GroupNorm2dDesc(Structure):
                 ("activation", c_int), ("eps", c_float)]
 
 
+class GroupNorm2dPlanInfo(Structure):
+    """struct spio_groupnorm_2d_plan_info."""
+
+    _fields_ = [(k, c_int) for k in ("one_launch", "threads", "smem_bytes", "slab_pieces", "slabs", "parts",
+                                     "cluster")] + [("grid", ctypes.c_uint), ("scratch_bytes", c_size_t)]
+
+    def as_dict(self):
+        return {name: getattr(self, name) for name, _ in self._fields_}
+
+
 class BackwardOpts(Structure):
     """struct spio_gw8_backward_opts."""
 
@@ -158,6 +168,8 @@ SIGNATURES = {
     "spio_layernorm_2d_bwd": (
         c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_longlong, c_int,
                 c_void_p, c_size_t, c_void_p]),
+    "spio_groupnorm_2d_plan_for": (
+        c_int, [POINTER(GroupNorm2dDesc), c_int, c_int, c_int, c_int, POINTER(GroupNorm2dPlanInfo)]),
     "spio_groupnorm_2d_fwd_scratch_bytes": (c_size_t, [POINTER(GroupNorm2dDesc)]),
     "spio_groupnorm_2d_fwd": (
         c_int, [c_void_p] * 7 + [POINTER(GroupNorm2dDesc), c_void_p, c_size_t, c_void_p]),

@@ -302,6 +302,7 @@ int choose_plan(const spio_groupnorm_2d_desc* d, const Device& dev, bool backwar
     sp = g.sp;
     set_many_parts(&g, dev, backward);
     set_ring(&p, d->type, bytes, backward);
+    if (p.smem > dev.smem) continue;
     const double cost = cost_of_two_launches(p, w, dev, backward);
     if (cost < least) least = cost, *best = p;
   }
@@ -403,6 +404,28 @@ int check_pointers(const spio_groupnorm_2d_desc* d, const void* out, const void*
 using namespace spio_b200;
 
 extern "C" {
+
+int spio_groupnorm_2d_plan_for(const spio_groupnorm_2d_desc* desc, int backward, int coded, int sm_count,
+                               int smem_optin_bytes, spio_groupnorm_2d_plan_info* info) {
+  if (check_desc(desc)) return 1;
+  if (info == nullptr) return jit_fail("info is NULL");
+  if (desc->n == 0 || desc->pixels == 0) return jit_fail("GroupNorm2d: nothing to plan for an empty tensor");
+  if (sm_count <= 0 || smem_optin_bytes <= 0) return jit_fail("GroupNorm2d: no such device");
+  const Device dev = {sm_count, smem_optin_bytes};
+  Plan p;
+  if (choose_plan(desc, dev, backward != 0, coded != 0, &p)) return 1;
+  *info = {};
+  info->one_launch = p.one_launch;
+  info->threads = p.threads;
+  info->smem_bytes = p.smem;
+  info->slab_pieces = p.g.sp;
+  info->slabs = p.g.slabs;
+  info->parts = p.g.parts;
+  info->cluster = p.g.cluster;
+  info->grid = p.grid;
+  info->scratch_bytes = backward ? p.channel_bytes + p.group_bytes : p.stats_bytes;
+  return 0;
+}
 
 size_t spio_groupnorm_2d_fwd_scratch_bytes(const spio_groupnorm_2d_desc* desc) {
   Device dev;

@@ -12,9 +12,49 @@ up to sum |x|, so its error is of the order 2^-24 * mean |x| after the division 
 mean of 0.02: four roundings of partial sums near 1 are 4 * 2^-24 = 2.4e-7, above 64 * 2^-24 * 0.045 = 1.7e-7.)
 """
 
+import ctypes
+
 import torch
 
+from spio_b200 import _clib
+
 CONST = 64 * 2.0 ** -24
+
+B200 = (148, 232448)  # multiprocessors, bytes of shared memory that a CTA may have
+
+# Sizes for which the planner takes a certain launch on a B200: (n, c, h, w), groups, type, activation, and the forms of the
+# forward pass, the forward pass that writes codes, the backward pass and the backward pass from codes: one launch or
+# two, `n` where the image's last slab of channels is narrower than the others.
+PLANNED = [
+    ((2, 24, 66, 55), 12, torch.float16, "relu", "1n 1n 1n 1n"),
+    ((4, 24, 42, 42), 3, torch.bfloat16, "relu", "1n 1n 1n 1n"),
+    ((3, 72, 28, 30), 9, torch.float32, "none", "1n 1n 1n 1n"),
+    ((1, 216, 42, 22), 108, torch.float32, "none", "1n 1n 1n 1n"),
+    ((1, 72, 81, 112), 6, torch.float16, "none", "1 1 2n 2n"),
+    ((1, 72, 118, 123), 36, torch.bfloat16, "relu", "1n 1n 2n 2n"),
+    ((1, 696, 35, 32), 6, torch.float32, "gelu", "2n 2n 2n 2n"),
+    ((1, 600, 39, 38), 3, torch.float32, "gelu", "2n 2n 2n 2n"),
+    ((1, 600, 48, 60), 24, torch.bfloat16, "gelu", "2n 2n 2n 2n"),
+    ((1, 72, 127, 166), 24, torch.bfloat16, "none", "2n 2n 2 2"),
+    ((1, 624, 59, 65), 3, torch.float16, "silu", "2n 2n 2 2"),
+    ((1, 744, 16, 15), 1, torch.float32, "gelu", "1 2 2 2"),
+    ((3, 568, 28, 21), 4, torch.bfloat16, "silu", "1 2 2 2"),
+    ((1, 40, 141, 178), 20, torch.float16, "silu", "1 2 2 2"),
+    ((1, 712, 16, 11), 4, torch.float32, "silu", "1 1 2 1"),
+    ((3, 24, 117, 119), 24, torch.bfloat16, "silu", "1n 1n 2 1n"),
+    ((4, 280, 63, 32), 10, torch.float32, "none", "1 1 1 2"),
+]
+
+
+def plan_of(shape, groups, dtype, act, backward=False, coded=False):
+    """What the library launches for these sizes on a B200."""
+    n, c, h, w = shape
+    types, acts = [torch.float16, torch.bfloat16, torch.float32], ["none", "relu", "silu", "gelu"]
+    desc = _clib.GroupNorm2dDesc(n, h * w, c, groups, types.index(dtype), acts.index(act), 1e-5)
+    info = _clib.GroupNorm2dPlanInfo()
+    _clib.check(_clib.load().spio_groupnorm_2d_plan_for(ctypes.byref(desc), backward, coded, *B200, ctypes.byref(info)),
+                "plan")
+    return info.as_dict()
 
 
 def half_step(t: torch.Tensor, dtype) -> torch.Tensor:

@@ -9,7 +9,7 @@ from torch import nn
 
 from spio_b200.functional import groupnorm_2d, groupnorm_2d_backward_op, groupnorm_2d_op
 from spio_b200.layers import GroupNorm2d
-from tests.norm_reference import CONST, Reference, assert_within
+from tests.norm_reference import CONST, PLANNED, Reference, assert_within
 
 pytestmark = pytest.mark.gpu
 CL = torch.channels_last
@@ -391,3 +391,11 @@ def test_clusters_one_behind_the_other(shape, groups):
         y, stats, _, _ = groupnorm_2d_op(x, w, b, groups, 1e-5, "silu", False)
         results.append((y, stats, *groupnorm_2d_backward_op(dy, x, None, None, stats, w, b, groups, "silu", True, True, True)))
     assert all(torch.equal(p, q) for r in results[1:] for p, q in zip(r, results[0]))
+
+
+@pytest.mark.parametrize("shape,groups,dtype,act,forms", PLANNED, ids=str)
+def test_every_form_of_launch(shape, groups, dtype, act, forms):
+    """One launch and two, the last slab of channels narrower or not, the same form for all passes or not (that these
+    sizes take those forms is tested without a GPU)."""
+    for checkpoint8 in (False, True):
+        check_all(shape, groups, dtype, act, checkpoint8, seed=27)

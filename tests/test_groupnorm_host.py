@@ -12,7 +12,7 @@ from spio_b200 import _clib
 from spio_b200.functional import (checkpoint8_pack, checkpoint8_unpack, conv2d_gw8_checkpoint8, groupnorm_2d,
                                   groupnorm_2d_op)
 from spio_b200.layers import GroupNorm2d
-from tests.norm_reference import blocks_of, restored
+from tests.norm_reference import B200, PLANNED, blocks_of, plan_of, restored
 
 
 def desc(n=2, pixels=12, c=32, groups=4, type=0, activation=0, eps=1e-5):
@@ -113,3 +113,30 @@ def test_reference_blocks():
     assert scale.item() == 1024 and set(codes.flatten().tolist()) == {63} and bool(restored(top).half().isfinite().all())
     codes, scale = blocks_of(torch.zeros(1, 8, 1, 1))
     assert scale.item() == 2.0 ** -126 and not bool(codes.any())
+
+
+@pytest.mark.parametrize("shape,groups,dtype,act,forms", PLANNED, ids=str)
+def test_forms_of_launch(shape, groups, dtype, act, forms):
+    """The sizes of the GPU test of this name reach what they are there for."""
+    for form, (backward, coded) in zip(forms.split(), ((0, 0), (0, 1), (1, 0), (1, 1))):
+        p = plan_of(shape, groups, dtype, act, backward, coded)
+        narrower = p["slab_pieces"] * p["slabs"] != shape[1] // 8
+        assert f"{2 - p['one_launch']}{'n' * narrower}" == form, (backward, coded, p)
+        # what any plan keeps to
+        assert p["parts"] % p["cluster"] == 0 and 1 <= p["cluster"] <= 16 and p["smem_bytes"] <= B200[1]
+        assert p["slab_pieces"] <= p["threads"] and 0 <= p["slab_pieces"] * p["slabs"] - shape[1] // 8 < p["slab_pieces"]
+        assert p["grid"] == shape[0] * p["slabs"] * p["parts"] and p["parts"] <= shape[2] * shape[3]
+        assert (p["slab_pieces"] * 8) % (shape[1] // groups) == 0          # whole groups
+        sums = 8 * shape[0] * p["parts"] * shape[1]                        # of the backward pass, for the channels
+        assert p["scratch_bytes"] >= sums if backward else (p["scratch_bytes"] > 0) == (p["one_launch"] == 0)
+
+
+def test_plan_refusals():
+    lib, info = _clib.load(), _clib.GroupNorm2dPlanInfo()
+    for d, sms, out, message in [(desc(groups=5), 148, info, "divisible"), (desc(n=0), 148, info, "empty"),
+                                 (desc(pixels=0), 148, info, "empty"), (desc(), 0, info, "device"), (desc(), 148, None, "NULL")]:
+        out = ctypes.byref(out) if out is not None else None
+        assert lib.spio_groupnorm_2d_plan_for(d, 0, 0, sms, B200[1], out) != 0 and message in _clib.last_error()
+    assert ctypes.sizeof(_clib.GroupNorm2dPlanInfo) == 8 * 4 + 8
+    for d in (desc(), desc(n=1, pixels=1 << 20)):      # too little shared memory for any launch
+        assert lib.spio_groupnorm_2d_plan_for(d, 0, 0, 148, 1024, ctypes.byref(info)) != 0 and "fits" in _clib.last_error()

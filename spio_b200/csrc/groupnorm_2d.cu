@@ -10,7 +10,9 @@
 #include <map>
 #include <mutex>
 #include <numeric>
+#include <set>
 #include <string>
+#include <utility>
 
 #include "cluster.cuh"
 #include "groupnorm_2d.h"
@@ -111,23 +113,36 @@ size_t aligned(size_t bytes) { return (bytes + 255) / 256 * 256; }
     if (e_ != cudaSuccess) return jit_fail(std::string("CUDA error: ") + cudaGetErrorString(e_)); \
   } while (0)
 
-// Lets a kernel have more than 48 KB of shared memory and clusters of more than 8 CTAs.
-int allow(const void* func, int smem, int cluster) {
-  if (smem > 48 * 1024) SPIO_CUDA(cudaFuncSetAttribute(func, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  if (cluster > 8) SPIO_CUDA(cudaFuncSetAttribute(func, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-  return 0;
-}
-
 struct Device {
   int sms, smem;  // multiprocessors, shared memory a block may have
+  int ordinal;
 };
 
 int device_of(Device* d) {
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&d->sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&d->smem, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev) != cudaSuccess)
+  if (cudaGetDevice(&d->ordinal) != cudaSuccess ||
+      cudaDeviceGetAttribute(&d->sms, cudaDevAttrMultiProcessorCount, d->ordinal) != cudaSuccess ||
+      cudaDeviceGetAttribute(&d->smem, cudaDevAttrMaxSharedMemoryPerBlockOptin, d->ordinal) != cudaSuccess)
     return jit_fail("CUDA error: no device");
+  return 0;
+}
+
+// Lets a kernel have more than 48 KB of shared memory and clusters of more than 8 CTAs.  The limits belong to the kernel
+// and the device, for all host threads: they are raised as far as they go, once, and never lowered to what one launch
+// needs, because a launch of another thread may be on its way that needs more.
+int allow(const void* func, const Device& dev) {
+  static std::mutex mutex;
+  static std::set<std::pair<const void*, int>> raised;
+  try {
+    std::lock_guard<std::mutex> lock(mutex);
+    if (raised.count({func, dev.ordinal})) return 0;
+    cudaFuncAttributes attr;
+    SPIO_CUDA(cudaFuncGetAttributes(&attr, func));
+    SPIO_CUDA(cudaFuncSetAttribute(func, cudaFuncAttributeMaxDynamicSharedMemorySize, dev.smem - (int)attr.sharedSizeBytes));
+    SPIO_CUDA(cudaFuncSetAttribute(func, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    raised.insert({func, dev.ordinal});
+  } catch (const std::exception& e) {  // no memory; C callers get an error like any other
+    return jit_fail(std::string("GroupNorm2d: ") + e.what());
+  }
   return 0;
 }
 
@@ -361,8 +376,8 @@ int make_plan(const spio_groupnorm_2d_desc* d, const Device& dev, bool backward,
   return 0;
 }
 
-int launch(const void* func, unsigned grid, int threads, int smem, int cluster, void* stream, void** args) {
-  if (allow(func, smem, cluster)) return 1;
+int launch(const void* func, const Device& dev, unsigned grid, int threads, int smem, int cluster, void* stream, void** args) {
+  if ((smem > 48 * 1024 || cluster > 8) && allow(func, dev)) return 1;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(threads);
@@ -411,7 +426,7 @@ int spio_groupnorm_2d_plan_for(const spio_groupnorm_2d_desc* desc, int backward,
   if (info == nullptr) return jit_fail("info is NULL");
   if (desc->n == 0 || desc->pixels == 0) return jit_fail("GroupNorm2d: nothing to plan for an empty tensor");
   if (sm_count <= 0 || smem_optin_bytes <= 0) return jit_fail("GroupNorm2d: no such device");
-  const Device dev = {sm_count, smem_optin_bytes};
+  const Device dev = {sm_count, smem_optin_bytes, -1};
   Plan p;
   if (choose_plan(desc, dev, backward != 0, coded != 0, &p)) return 1;
   *info = {};
@@ -449,13 +464,13 @@ int spio_groupnorm_2d_fwd(void* y, float* stats, void* codes, void* exponents, c
   const GnKernels* k = kernels_of(desc->type, p.threads == kGnWide);
   if (p.one_launch) {
     void* args[] = {&y, &stats, &codes, &exponents, (void*)&x, (void*)&weight, (void*)&bias, &p.g};
-    return launch(k->fwd[desc->activation][coded], p.grid, p.threads, p.smem, p.g.cluster, stream, args);
+    return launch(k->fwd[desc->activation][coded], dev, p.grid, p.threads, p.smem, p.g.cluster, stream, args);
   }
   if (scratch == nullptr || scratch_bytes < p.stats_bytes) return jit_fail("GroupNorm2d scratch buffer is too small");
   void* sargs[] = {&scratch, (void*)&x, &p.g};
-  if (launch(k->stats, p.grid, p.threads, p.smem, p.g.cluster, stream, sargs)) return 1;
+  if (launch(k->stats, dev, p.grid, p.threads, p.smem, p.g.cluster, stream, sargs)) return 1;
   void* args[] = {&y, &stats, &codes, &exponents, (void*)&x, (void*)&weight, (void*)&bias, &scratch, &p.g};
-  return launch(k->apply[desc->activation][coded], p.grid, p.threads, p.smem, 1, stream, args);
+  return launch(k->apply[desc->activation][coded], dev, p.grid, p.threads, p.smem, 1, stream, args);
 }
 
 size_t spio_groupnorm_2d_bwd_scratch_bytes(const spio_groupnorm_2d_desc* desc) {
@@ -494,16 +509,16 @@ int spio_groupnorm_2d_bwd(void* dx, float* dweight, float* dbias, const void* dy
   if (p.one_launch) {
     void* args[] = {&dx, &part_channel, (void*)&dy, (void*)&x, (void*)&codes, (void*)&exponents,
                     (void*)&stats, (void*)&weight, (void*)&bias, &p.g};
-    if (launch(k->bwd[desc->activation][coded], p.grid, p.threads, p.smem, p.g.cluster, stream, args)) return 1;
+    if (launch(k->bwd[desc->activation][coded], dev, p.grid, p.threads, p.smem, p.g.cluster, stream, args)) return 1;
   } else {
     float2* part_group = dx != nullptr ? reinterpret_cast<float2*>(static_cast<char*>(scratch) + p.channel_bytes) : nullptr;
     void* args[] = {&part_channel, &part_group, (void*)&dy, (void*)&x, (void*)&codes, (void*)&exponents,
                     (void*)&stats, (void*)&weight, (void*)&bias, &p.g};
-    if (launch(k->bwd_sums[desc->activation][coded], p.grid, p.threads, p.smem, p.g.cluster, stream, args)) return 1;
+    if (launch(k->bwd_sums[desc->activation][coded], dev, p.grid, p.threads, p.smem, p.g.cluster, stream, args)) return 1;
     if (dx != nullptr) {
       void* dargs[] = {&dx, &part_group, (void*)&dy, (void*)&x, (void*)&codes, (void*)&exponents,
                        (void*)&stats, (void*)&weight, (void*)&bias, &p.g};
-      if (launch(k->bwd_apply[desc->activation][coded], p.grid, p.threads, p.smem, 1, stream, dargs)) return 1;
+      if (launch(k->bwd_apply[desc->activation][coded], dev, p.grid, p.threads, p.smem, 1, stream, dargs)) return 1;
     }
   }
   if (sums) {
@@ -512,7 +527,7 @@ int spio_groupnorm_2d_bwd(void* dx, float* dweight, float* dbias, const void* dy
     while (rows > 1024 && split < 8 && rows / 256 > split) split *= 2;
     void* rargs[] = {&dweight, &dbias, &part_channel, &c, &rows, &split};
     const void* reduce = split > 1 ? (const void*)&groupnorm_2d_bwd_reduce_kernel<true> : (const void*)&groupnorm_2d_bwd_reduce_kernel<false>;
-    return launch(reduce, (2 * c + 31) / 32 * split, 1024, 0, split, stream, rargs);
+    return launch(reduce, dev, (2 * c + 31) / 32 * split, 1024, 0, split, stream, rargs);
   }
   return 0;
 }

@@ -2,6 +2,7 @@
 layouts, streams and CUDA graphs, against the definition in float64."""
 
 import itertools
+import threading
 
 import pytest
 import torch
@@ -9,7 +10,7 @@ from torch import nn
 
 from spio_b200.functional import groupnorm_2d, groupnorm_2d_backward_op, groupnorm_2d_op
 from spio_b200.layers import GroupNorm2d
-from tests.norm_reference import CONST, PLANNED, Reference, assert_within
+from tests.norm_reference import CONST, PLANNED, Reference, assert_within, plan_of
 
 pytestmark = pytest.mark.gpu
 CL = torch.channels_last
@@ -399,3 +400,34 @@ def test_every_form_of_launch(shape, groups, dtype, act, forms):
     sizes take those forms is tested without a GPU)."""
     for checkpoint8 in (False, True):
         check_all(shape, groups, dtype, act, checkpoint8, seed=27)
+
+
+def test_two_threads_that_share_a_kernel():
+    """Host threads that launch one kernel with different amounts of shared memory, each on a stream of its own."""
+    sizes = [((4, 256, 20, 20), 256), ((4, 96, 40, 40), 3)]
+    for backward in (False, True):
+        plans = [plan_of(s, g, torch.float16, "relu", backward) for s, g in sizes]
+        assert all(p["one_launch"] and p["smem_bytes"] > 48 * 1024 for p in plans)
+        assert plans[0]["threads"] == plans[1]["threads"] and plans[0]["smem_bytes"] != plans[1]["smem_bytes"], plans
+    data = [make(s, torch.float16, seed=31) for s, _ in sizes]
+    once = lambda x, dy, w, b, g: (lambda y, st: (y, *groupnorm_2d_backward_op(dy, x, None, None, st, w, b, g, "relu", True,  # noqa: E731
+                                                                               True, True)))(*groupnorm_2d_op(x, w, b, g, 1e-5, "relu", False)[:2])
+    want = [once(*d, g) for d, (_, g) in zip(data, sizes)]
+    torch.cuda.synchronize()
+    failures, start = [], threading.Barrier(4)
+
+    def work(i):
+        try:
+            stream = torch.cuda.Stream()
+            start.wait(timeout=60)
+            with torch.cuda.stream(stream):
+                for _ in range(400):
+                    got = once(*data[i % 2], sizes[i % 2][1])
+            stream.synchronize()
+            assert all(torch.equal(p, q) for p, q in zip(got, want[i % 2]))
+        except Exception as e:      # noqa: BLE001
+            failures.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    [t.start() for t in threads], [t.join() for t in threads]
+    assert not failures, failures[0]

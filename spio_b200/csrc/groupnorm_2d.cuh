@@ -82,7 +82,10 @@ struct Activation {
   // grad * act'(z)
   static __device__ __forceinline__ Pair back(Pair grad, Pair z) {
     const float2 f = unpair(z);
-    if (ACT == kActRelu) return grad * pair(f.x <= 0.f ? 0.f : 1.f, f.y <= 0.f ? 0.f : 1.f);
+    if (ACT == kActRelu) {  // chosen, not multiplied: an infinite gradient where ReLU is off counts for nothing
+      const float2 d = unpair(grad);
+      return pair(f.x <= 0.f ? 0.f : d.x, f.y <= 0.f ? 0.f : d.y);
+    }
     if (ACT == kActSilu) {
       const Pair s = EXACT ? pair(exact_sigmoid(f.x), exact_sigmoid(f.y)) : sigmoid(z);
       return grad * fma2(z * s, fma2(s, pair(-1.f), pair(1.f)), s);

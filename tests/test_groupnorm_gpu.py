@@ -431,3 +431,25 @@ def test_two_threads_that_share_a_kernel():
     threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
     [t.start() for t in threads], [t.join() for t in threads]
     assert not failures, failures[0]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("shape,groups", [((3, 32, 9, 8), 4), ((2, 48, 10, 9), 16), ((1, 696, 35, 32), 6)], ids=str)
+@pytest.mark.parametrize("checkpoint8", [False, True])
+def test_nonfinite_gradients_where_relu_is_off(dtype, shape, groups, checkpoint8):
+    """ReLU selects: an infinite or NaN gradient at a place that it has set to zero is left out, as by torch's layers."""
+    x, dy, w, b = make(shape, dtype, seed=28)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    y = groupnorm_2d(x, groups, w, b, activation="relu", checkpoint8=checkpoint8)
+    z = nn.functional.group_norm(x.detach().double(), groups, w.detach().double(), b.detach().double())
+    flat = lambda t: t.permute(0, 2, 3, 1).reshape(-1)  # noqa: E731  (a view: channels_last)
+    off = flat(z).argsort()[:3]                             # far below zero, from the input's 8-bit form too
+    assert not bool(flat(y)[off].any()) and float(flat(z)[off].max()) < -1
+    flat(dy)[off] = 0
+    want = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+    flat(dy)[off] = torch.tensor([float("inf"), float("-inf"), float("nan")], device="cuda", dtype=dtype)
+    got = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+    assert all(bool(p.isfinite().all()) and torch.equal(p, q) for p, q in zip(got, want))
+    on = int(flat(z).argmax())                              # where ReLU is on it still shows
+    flat(dy)[on] = float("inf")
+    assert not bool(torch.autograd.grad(y, leaves, dy)[0].isfinite().all())

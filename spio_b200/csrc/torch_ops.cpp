@@ -236,6 +236,44 @@ auto infer_op() {
 OptTensor optional_of(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
 Tensor tensor_of(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
 
+// Forward-mode derivatives: refused, or the result would seem constant.
+void check_no_tangent(const Tensor& t, const char* what = "groupnorm_2d") {
+  TORCH_CHECK(!t._fw_grad(0).defined(), "spio ", what, " has no forward-mode derivative");
+}
+void check_no_tangent(const OptTensor& t) {
+  if (t.has_value()) check_no_tangent(*t);
+}
+
+// The backward operator refuses a derivative of its own instead of returning values that seem constant.  `origin`: a
+// tensor at the place in the graph of what the gradients depend on besides.
+struct GroupNormBackward : torch::autograd::Function<GroupNormBackward> {
+  static variable_list forward(torch::autograd::AutogradContext*, const Tensor& dy, const OptTensor& x,
+                               const OptTensor& codes, const OptTensor& exponents, const Tensor& stats,
+                               const OptTensor& weight, const OptTensor& bias,
+                               int64_t num_groups, std::string activation, bool needs_input_grad,
+                               bool needs_weight_grad, bool needs_bias_grad, const OptTensor&) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [dx, dw, db] = backward_op().call(dy, x, codes, exponents, stats, weight, bias, num_groups, activation,
+                                           needs_input_grad, needs_weight_grad, needs_bias_grad);
+    return {dx, dw, db};
+  }
+  static variable_list backward(torch::autograd::AutogradContext*, const variable_list&) {
+    TORCH_CHECK(false, "spio groupnorm_2d cannot be differentiated twice");
+  }
+};
+
+// An empty tensor at the place in the graph of the first input of the backward node that is running (where that requires
+// a gradient).
+OptTensor origin_of_input() {
+  const auto node = torch::autograd::get_current_node();
+  TORCH_CHECK(node, "spio groupnorm_2d cannot be differentiated twice");
+  const torch::autograd::Edge edge = node->next_edge(0);
+  if (!edge.is_valid()) return std::nullopt;
+  const Tensor t = at::empty({0});
+  torch::autograd::impl::set_gradient_edge(t, edge);
+  return t;
+}
+
 struct GroupNorm : torch::autograd::Function<GroupNorm> {
   static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const OptTensor& weight,
                         const OptTensor& bias, int64_t num_groups, double eps, std::string activation, bool checkpoint8) {
@@ -252,6 +290,7 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
     const variable_list saved = ctx->get_saved_variables();
     variable_list result(7);
     if (!grads[0].defined()) return result;
+    check_no_tangent(grads[0]);
     // (an absent weight or bias has no edge in the graph)
     size_t edge = 0;
     const bool want_x = ctx->needs_input_grad(edge++);
@@ -259,8 +298,17 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
     const bool want_bias = saved[5].defined() && ctx->needs_input_grad(edge++);
     const bool want[3] = {want_x, want_weight, want_bias};
     const int64_t call = ctx->saved_data["call"].toInt();
-    std::optional<at::AutoDispatchBelowADInplaceOrView> below;  // (with grad mode on, the operator refuses what it has to)
-    if (!at::GradMode::is_enabled()) below.emplace();
+    if (at::GradMode::is_enabled()) {  // a derivative of the gradients may be asked for, which the node refuses;
+      // the 8-bit form of x is no part of the graph, x itself is
+      const variable_list r = GroupNormBackward::apply(
+          grads[0], optional_of(saved[0]), optional_of(saved[1]), optional_of(saved[2]), saved[3], optional_of(saved[4]),
+          optional_of(saved[5]), call / kActivations, std::string(kActivationNames[call % kActivations]), want[0], want[1],
+          want[2], saved[1].defined() ? origin_of_input() : std::nullopt);
+      for (int i = 0; i < 3; ++i)
+        if (want[i]) result[i] = r[i];
+      return result;
+    }
+    at::AutoDispatchBelowADInplaceOrView below;
     auto [dx, dw, db] = backward_op().call(
         grads[0], optional_of(saved[0]), optional_of(saved[1]), optional_of(saved[2]), saved[3], optional_of(saved[4]),
         optional_of(saved[5]), call / kActivations, kActivationNames[call % kActivations], want[0], want[1], want[2]);
@@ -273,14 +321,6 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
 
 bool requires_grad(const OptTensor& t) { return t.has_value() && t->requires_grad(); }
 
-// Forward-mode derivatives: refused, or the result would seem constant.
-void check_no_tangent(const Tensor& t) {
-  TORCH_CHECK(!t._fw_grad(0).defined(), "spio groupnorm_2d has no forward-mode derivative");
-}
-void check_no_tangent(const OptTensor& t) {
-  if (t.has_value()) check_no_tangent(*t);
-}
-
 Tensor groupnorm_2d_autograd(const Tensor& x, const OptTensor& weight, const OptTensor& bias, int64_t num_groups,
                              double eps, c10::string_view activation, bool checkpoint8) {
   check_no_tangent(x), check_no_tangent(weight), check_no_tangent(bias);
@@ -290,23 +330,6 @@ Tensor groupnorm_2d_autograd(const Tensor& x, const OptTensor& weight, const Opt
   return infer_op().call(x, weight, bias, num_groups, eps, activation, checkpoint8);
 }
 
-// The backward operator refuses a derivative of its own instead of returning values that seem constant.
-struct GroupNormBackward : torch::autograd::Function<GroupNormBackward> {
-  static variable_list forward(torch::autograd::AutogradContext*, const Tensor& dy, const OptTensor& x,
-                               const OptTensor& codes, const OptTensor& exponents, const Tensor& stats,
-                               const OptTensor& weight, const OptTensor& bias,
-                               int64_t num_groups, std::string activation, bool needs_input_grad,
-                               bool needs_weight_grad, bool needs_bias_grad) {
-    at::AutoDispatchBelowADInplaceOrView below;
-    auto [dx, dw, db] = backward_op().call(dy, x, codes, exponents, stats, weight, bias, num_groups, activation,
-                                           needs_input_grad, needs_weight_grad, needs_bias_grad);
-    return {dx, dw, db};
-  }
-  static variable_list backward(torch::autograd::AutogradContext*, const variable_list&) {
-    TORCH_CHECK(false, "spio groupnorm_2d cannot be differentiated twice");
-  }
-};
-
 std::tuple<Tensor, Tensor, Tensor> groupnorm_2d_backward_autograd(
     const Tensor& dy, const OptTensor& x, const OptTensor& codes, const OptTensor& exponents, const Tensor& stats,
     const OptTensor& weight, const OptTensor& bias, int64_t num_groups, c10::string_view activation,
@@ -315,7 +338,7 @@ std::tuple<Tensor, Tensor, Tensor> groupnorm_2d_backward_autograd(
   if (at::GradMode::is_enabled() && (dy.requires_grad() || requires_grad(x) || requires_grad(weight) || requires_grad(bias))) {
     const variable_list r =
         GroupNormBackward::apply(dy, x, codes, exponents, stats, weight, bias, num_groups, std::string(activation),
-                                 needs_input_grad, needs_weight_grad, needs_bias_grad);
+                                 needs_input_grad, needs_weight_grad, needs_bias_grad, std::nullopt);
     return {r[0], r[1], r[2]};
   }
   at::AutoDispatchBelowADInplaceOrView below;
@@ -398,6 +421,7 @@ struct ConvCheckpoint8 : torch::autograd::Function<ConvCheckpoint8> {
     const variable_list saved = ctx->get_saved_variables();
     variable_list result(6);
     if (!grads[0].defined()) return result;
+    check_no_tangent(grads[0], "conv2d_gw8_checkpoint8");
     const Tensor &codes = saved[0], &exponents = saved[1], &weight = saved[2];
     const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
     const bool want_b = saved[3].defined() && ctx->needs_input_grad(2);

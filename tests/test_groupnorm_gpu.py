@@ -8,7 +8,7 @@ import pytest
 import torch
 from torch import nn
 
-from spio_b200.functional import groupnorm_2d, groupnorm_2d_backward_op, groupnorm_2d_op
+from spio_b200.functional import conv2d_gw8_checkpoint8, groupnorm_2d, groupnorm_2d_backward_op, groupnorm_2d_op
 from spio_b200.layers import GroupNorm2d
 from tests.norm_reference import CONST, PLANNED, Reference, assert_within, plan_of
 
@@ -453,3 +453,44 @@ def test_nonfinite_gradients_where_relu_is_off(dtype, shape, groups, checkpoint8
     on = int(flat(z).argmax())                              # where ReLU is on it still shows
     flat(dy)[on] = float("inf")
     assert not bool(torch.autograd.grad(y, leaves, dy)[0].isfinite().all())
+
+
+@pytest.mark.parametrize("affine", ["none", "frozen", "trained"])
+@pytest.mark.parametrize("checkpoint8", [False, True])
+@pytest.mark.parametrize("inner", [False, True])
+def test_a_gradient_term_is_refused_and_not_lost(affine, checkpoint8, inner):
+    """A penalty on the input's gradient, which would need the second derivative: whatever requires a gradient beside the
+    input, and whether or not the input is a leaf."""
+    leaf, dy, w, b = make((2, 16, 4, 4), torch.float32, seed=29)
+    leaf.requires_grad_(True)
+    x = leaf * 2 if inner else leaf
+    if affine == "none":
+        w = b = None
+    elif affine == "trained":
+        w.requires_grad_(True), b.requires_grad_(True)
+    y = groupnorm_2d(x, 4, w, b, activation="silu", checkpoint8=checkpoint8)
+    first = torch.autograd.grad(y, x, dy, retain_graph=True)[0]
+    (dx,) = torch.autograd.grad(y, x, dy, create_graph=True)
+    assert torch.equal(dx, first)                      # the first derivative is there
+    with pytest.raises(RuntimeError, match="twice"):
+        (y.sum() + dx.square().sum()).backward(retain_graph=True)
+    with pytest.raises(RuntimeError, match="twice"):
+        torch.autograd.grad(dx.square().sum(), leaf, allow_unused=True)
+
+
+@pytest.mark.parametrize("checkpoint8", [False, True])
+@pytest.mark.parametrize("create_graph", [False, True])
+def test_a_tangent_of_the_output_gradient_is_refused_and_not_lost(checkpoint8, create_graph):
+    """Forward over reverse: the gradients would come back without their tangents."""
+    x, dy, w, b = make((2, 16, 4, 4), torch.float32, seed=32)
+    y = groupnorm_2d(x.requires_grad_(True), 4, w, b, checkpoint8=checkpoint8)
+    weight = torch.randn(16, 8, 3, 3, device="cuda").half().requires_grad_(True)
+    c = conv2d_gw8_checkpoint8(x.detach().half(), weight, None, padding_y=1, padding_x=1, groups=2)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(dy, torch.ones_like(dy))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(y, x, dual, create_graph=create_graph)
+        if checkpoint8:
+            dual = torch.autograd.forward_ad.make_dual(dy.half(), torch.ones_like(dy).half())
+            with pytest.raises(RuntimeError, match="twice" if create_graph else "forward-mode"):
+                torch.autograd.grad(c, weight, dual, create_graph=create_graph)

@@ -109,6 +109,14 @@ Tensor checkpoint8_unpack(const Tensor& codes_, const Tensor& exponents_, at::Sc
 
 // ---------------------------------------------------------------- group norm
 
+// (No sizes: these may be symbolic while a call is traced.)
+void check_parameter_types(const Tensor& x, const OptTensor& weight, const OptTensor& bias) {
+  const auto both = [&](at::ScalarType type) {
+    return (!weight.has_value() || weight->scalar_type() == type) && (!bias.has_value() || bias->scalar_type() == type);
+  };
+  TORCH_CHECK_VALUE(both(at::kFloat) || both(x.scalar_type()), "weight and bias are both fp32 or both of the data's type");
+}
+
 spio_groupnorm_2d_desc describe(const Tensor& x, const OptTensor& weight, const OptTensor& bias, int64_t num_groups,
                                 double eps, c10::string_view activation) {
   check_image(x, "groupnorm_2d");
@@ -117,9 +125,10 @@ spio_groupnorm_2d_desc describe(const Tensor& x, const OptTensor& weight, const 
   TORCH_CHECK_VALUE(num_groups > 0 && c % num_groups == 0, "Number of channels must be divisible by the number of groups.");
   TORCH_CHECK_VALUE(c <= (1 << 20), "GroupNorm2d supports at most 2^20 channels");
   TORCH_CHECK_VALUE(eps >= 0, "eps must not be negative");
+  check_parameter_types(x, weight, bias);
   for (const OptTensor* t : {&weight, &bias})
-    TORCH_CHECK_VALUE(!t->has_value() || ((*t)->scalar_type() == at::kFloat && (*t)->dim() == 1 && (*t)->numel() == c && (*t)->device() == x.device()),
-                      "weight and bias are fp32 vectors of the channels on the data's device");
+    TORCH_CHECK_VALUE(!t->has_value() || ((*t)->dim() == 1 && (*t)->numel() == c && (*t)->device() == x.device()),
+                      "weight and bias are vectors of the channels on the data's device");
   spio_groupnorm_2d_desc d;
   d.n = x.size(0);
   d.pixels = x.size(2) * x.size(3);
@@ -131,7 +140,9 @@ spio_groupnorm_2d_desc describe(const Tensor& x, const OptTensor& weight, const 
   return d;
 }
 
-Tensor vector_of(const OptTensor& t) { return t.has_value() ? t->contiguous() : Tensor(); }
+// In fp32, as the kernels take them (a 16-bit vector is exact in it).
+OptTensor fp32(const OptTensor& t) { return t.has_value() ? OptTensor(t->to(at::kFloat)) : std::nullopt; }
+Tensor vector_of(const OptTensor& t) { return t.has_value() ? t->to(at::kFloat).contiguous() : Tensor(); }
 
 Tensor scratch_of(size_t bytes, const Tensor& like) {
   return bytes > 0 ? empty_vector((int64_t)bytes, like, at::kByte) : Tensor();
@@ -324,8 +335,11 @@ bool requires_grad(const OptTensor& t) { return t.has_value() && t->requires_gra
 Tensor groupnorm_2d_autograd(const Tensor& x, const OptTensor& weight, const OptTensor& bias, int64_t num_groups,
                              double eps, c10::string_view activation, bool checkpoint8) {
   check_no_tangent(x), check_no_tangent(weight), check_no_tangent(bias);
-  if (at::GradMode::is_enabled() && (x.requires_grad() || requires_grad(weight) || requires_grad(bias)))
-    return GroupNorm::apply(x, weight, bias, num_groups, eps, std::string(activation), checkpoint8);
+  if (at::GradMode::is_enabled() && (x.requires_grad() || requires_grad(weight) || requires_grad(bias))) {
+    check_parameter_types(x, weight, bias);
+    // 16-bit parameters: their gradients are rounded to their type once, by the derivative of this conversion
+    return GroupNorm::apply(x, fp32(weight), fp32(bias), num_groups, eps, std::string(activation), checkpoint8);
+  }
   at::AutoDispatchBelowADInplaceOrView below;
   return infer_op().call(x, weight, bias, num_groups, eps, activation, checkpoint8);
 }
@@ -352,7 +366,6 @@ std::tuple<Tensor, Tensor, Tensor> groupnorm_2d_backward_autograd(
 Tensor groupnorm_2d_autocast(const Tensor& x, const OptTensor& weight, const OptTensor& bias, int64_t num_groups,
                              double eps, c10::string_view activation, bool checkpoint8) {
   const c10::impl::ExcludeDispatchKeyGuard no_autocast(c10::DispatchKey::AutocastCUDA);
-  const auto fp32 = [](const OptTensor& t) { return t.has_value() ? OptTensor(t->to(at::kFloat)) : std::nullopt; };
   return infer_op().call(x, fp32(weight), fp32(bias), num_groups, eps, activation, checkpoint8);
 }
 

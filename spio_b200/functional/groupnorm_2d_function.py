@@ -3,7 +3,7 @@ with an affine map and an activation, forward and backward.
 
     z = (x - mean) * rstd * weight + bias,   y = activation(z)
 
-Data is float16, bfloat16 or float32; statistics, weight and bias are fp32.  With ``checkpoint8`` the forward pass
+Data is float16, bfloat16 or float32; statistics are fp32, weight and bias too or of the data's type.  With ``checkpoint8`` the forward pass
 writes the 8-bit form of its input beside the output (see ``checkpoint8_function``) and the backward pass reads that
 instead of the input.  The reference has no group norm.  The device work is done by libspio_b200 on torch's
 current stream; CPU tensors raise.
@@ -70,8 +70,8 @@ def groupnorm_2d(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor
     """``activation(group_norm(x))`` of an NCHW tensor (channels_last on a CUDA device; float16, bfloat16 or
     float32, a multiple of 8 channels).
 
-    ``weight`` and ``bias`` are fp32 vectors of the channels (of any type under autocast, where the data keeps its
-    own); ``activation`` is ``"none"``, ``"relu"``, ``"silu"`` or ``"gelu"`` (with the error function).  A group, rounded
+    ``weight`` and ``bias`` are vectors of the channels, both fp32 or both of the data's type (of any type under
+    autocast, where the data keeps its own); they are taken in fp32, and their gradients are rounded once.  ``activation`` is ``"none"``, ``"relu"``, ``"silu"`` or ``"gelu"`` (with the error function).  A group, rounded
     up to whole blocks of 8 channels, may span at most 2048 channels.  ``checkpoint8`` keeps the 8-bit form of
     ``x`` for the backward pass instead of ``x`` (1.125 bytes a value): the gradients are then taken at the
     restored values, with the statistics of ``x`` itself."""

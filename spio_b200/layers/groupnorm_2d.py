@@ -1,5 +1,6 @@
 """``GroupNorm2d``: group norm with an activation over an NCHW tensor, backed by the ``spio::groupnorm_2d`` operator
-(channels_last float16, bfloat16 or float32 data on a CUDA device; fp32 parameters)."""
+(channels_last float16, bfloat16 or float32 data on a CUDA device; parameters in fp32 or of the data's type, of any type
+under autocast)."""
 
 from __future__ import annotations
 

@@ -10,7 +10,8 @@ from torch import nn
 
 from spio_b200.functional import conv2d_gw8_checkpoint8, groupnorm_2d, groupnorm_2d_backward_op, groupnorm_2d_op
 from spio_b200.layers import GroupNorm2d
-from tests.norm_reference import CONST, PLANNED, Reference, assert_within, plan_of
+from spio_b200.transform import transform
+from tests.norm_reference import CONST, PLANNED, Reference, assert_within, half_step, plan_of
 
 pytestmark = pytest.mark.gpu
 CL = torch.channels_last
@@ -494,3 +495,43 @@ def test_a_tangent_of_the_output_gradient_is_refused_and_not_lost(checkpoint8, c
             dual = torch.autograd.forward_ad.make_dual(dy.half(), torch.ones_like(dy).half())
             with pytest.raises(RuntimeError, match="twice" if create_graph else "forward-mode"):
                 torch.autograd.grad(c, weight, dual, create_graph=create_graph)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("checkpoint8", [False, True])
+def test_model_held_in_16_bits(dtype, checkpoint8):
+    """A model cast to fp16 or bf16, outside autocast: parameters of the data's type are taken in fp32, their gradients
+    come back in their own type (one rounding)."""
+    shape, groups = (3, 64, 9, 7), 8
+    x, dy, w, b = make(shape, dtype, seed=30)
+    model = nn.Sequential(nn.GroupNorm(groups, 64), nn.SiLU()).cuda()
+    with torch.no_grad():
+        model[0].weight.copy_(w), model[0].bias.copy_(b)
+    model.to(dtype)
+    weight, bias = model[0].weight, model[0].bias
+    ref = Reference(x, groups, weight, bias, 1e-5, "silu", dy, checkpoint8)
+    for fast in (transform(model, group_norm=True, checkpoint8=checkpoint8),
+                 GroupNorm2d.from_torch_module(model[0], "silu", checkpoint8)):
+        xs = x.clone().requires_grad_(True)
+        y = fast(xs)
+        assert y.dtype == dtype
+        assert_within(y, ref.y, ref.y_tol, "y")
+        dx, dw, db = torch.autograd.grad(y, (xs, weight, bias), dy)
+        assert_within(dx, ref.dx, ref.dx_tol, "dx")
+        assert dw.dtype == db.dtype == dtype
+        assert_within(dw, ref.dweight, ref.dweight_tol + half_step(ref.dweight.abs() + ref.dweight_tol, dtype), "dweight")
+        assert_within(db, ref.dbias, ref.dbias_tol + half_step(ref.dbias.abs() + ref.dbias_tol, dtype), "dbias")
+        with torch.inference_mode():
+            assert torch.equal(fast(x), y)
+        with torch.no_grad():
+            assert torch.equal(fast(x), y)
+    layer = GroupNorm2d(groups, 64, dtype=dtype, device="cuda")
+    assert torch.equal(layer(x), groupnorm_2d(x, groups))
+    assert torch.equal(groupnorm_2d(x, groups, weight, None), groupnorm_2d(x, groups, weight.float(), None))
+    # neither types that differ from each other nor a 16-bit vector beside data of another type
+    other = torch.bfloat16 if dtype is torch.float16 else torch.float16
+    for call in (lambda: groupnorm_2d(x, groups, weight, bias.float()), lambda: groupnorm_2d(x, groups, weight.float(), bias),
+                 lambda: groupnorm_2d(x.float(), groups, weight, bias), lambda: groupnorm_2d(x.to(other), groups, weight, bias),
+                 lambda: groupnorm_2d(x, groups, weight.double(), bias.double())):
+        with pytest.raises(ValueError, match="weight and bias"):
+            call()

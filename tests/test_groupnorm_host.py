@@ -140,3 +140,15 @@ def test_plan_refusals():
     assert ctypes.sizeof(_clib.GroupNorm2dPlanInfo) == 8 * 4 + 8
     for d in (desc(), desc(n=1, pixels=1 << 20)):      # too little shared memory for any launch
         assert lib.spio_groupnorm_2d_plan_for(d, 0, 0, 148, 1024, ctypes.byref(info)) != 0 and "fits" in _clib.last_error()
+
+
+def test_parameter_types_under_fake_tensors():
+    """16-bit parameters beside data of their type are taken, other mixtures refused."""
+    with FakeTensorMode():
+        x = torch.empty(2, 32, 5, 7, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+        w = torch.ones(32, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+        y = groupnorm_2d(x, 4, w, w, activation="silu", checkpoint8=True)
+        assert y.requires_grad and y.dtype == torch.bfloat16
+        for weight, bias in ((w, w.float()), (w.half(), None), (None, w.double())):
+            with pytest.raises(ValueError, match="weight and bias"):
+                groupnorm_2d(x, 4, weight, bias)

@@ -1,7 +1,10 @@
 """spio_b200: B200-native (sm_100a) grouped conv2d with group width 8.
 
 Importing the package touches neither CUDA nor the native library; both are loaded on
-first use (the reference initialises the driver at import, spio/__init__.py:8-14).
+first use (the reference initialises the driver at import, spio/__init__.py:8-14).  Importing
+``spio_b200.functional``, or what uses it, also loads the library with the PyTorch operators in C++
+where that fits the installed torch; it initialises no device either, and where it does not fit,
+only the calls of those operators fail.
 """
 
 __version__ = "0.2.0"

@@ -15,6 +15,8 @@ from typing import Optional
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libspio_b200.so"
 
 TORCH_LIB_PATH = LIB_PATH.with_name("libspio_b200_torch.so")
+# beside it, what torch it was compiled against: it uses torch's C++ interface, which changes between versions
+TORCH_STAMP_PATH = TORCH_LIB_PATH.with_suffix(".built_for")
 
 FPROP, DGRAD, WGRAD = 0, 1, 2
 
@@ -215,6 +217,13 @@ def load() -> ctypes.CDLL:
 _torch_ops_loaded = False
 
 
+def torch_stamp() -> str:
+    """The installed torch, as the build records it."""
+    import torch
+
+    return f"torch {torch.__version__} cxx11_abi={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"
+
+
 def load_torch_ops() -> None:
     """Load the library with the operators that are implemented in C++ (csrc/torch_ops.cpp) once."""
     global _torch_ops_loaded
@@ -222,12 +231,27 @@ def load_torch_ops() -> None:
         return
     import torch
 
+    again = "build it with `python -m spio_b200.build` (there is no fallback implementation)"
     for path in (LIB_PATH, TORCH_LIB_PATH):
         if not path.exists():
-            raise RuntimeError(f"{path} is missing: build it with `python -m spio_b200.build` "
-                               "(there is no fallback implementation)")
-    torch.ops.load_library(str(TORCH_LIB_PATH))
+            raise RuntimeError(f"{path} is missing: {again}")
+    if TORCH_STAMP_PATH.exists() and TORCH_STAMP_PATH.read_text().strip() != torch_stamp():
+        raise RuntimeError(f"{TORCH_LIB_PATH} was built for {TORCH_STAMP_PATH.read_text().strip()} and {torch_stamp()} is "
+                           f"installed: {again}")
+    try:
+        torch.ops.load_library(str(TORCH_LIB_PATH))
+    except OSError as e:
+        raise RuntimeError(f"{TORCH_LIB_PATH} does not load with {torch_stamp()} ({e}): {again}") from e
     _torch_ops_loaded = True
+
+
+def load_torch_ops_if_usable() -> None:
+    """The same where it can be done; where not, the operators' own calls say why.  (For imports: what else the package
+    offers does not need that library.)"""
+    try:
+        load_torch_ops()
+    except RuntimeError:
+        pass
 
 
 def last_error() -> str:

@@ -14,13 +14,15 @@ import subprocess
 import sys
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
+from typing import Optional
+
+from ._clib import TORCH_LIB_PATH, TORCH_STAMP_PATH, torch_stamp
 
 PKG_DIR = Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
 LIB_DIR = PKG_DIR / "lib"
 OBJ_DIR = PKG_DIR / "lib" / "obj"
 LIB_PATH = LIB_DIR / "libspio_b200.so"
-TORCH_LIB_PATH = LIB_DIR / "libspio_b200_torch.so"
 TORCH_SOURCE = CSRC / "torch_ops.cpp"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -72,9 +74,11 @@ def is_current() -> bool:
 
 
 def torch_lib_is_current() -> bool:
+    """Whether it is newer than what it is made from, and made for the installed torch."""
     header = PKG_DIR.parent / "include" / "spio_b200.h"
     newest = max(p.stat().st_mtime for p in (TORCH_SOURCE, header))
-    return TORCH_LIB_PATH.exists() and TORCH_LIB_PATH.stat().st_mtime >= newest
+    return (TORCH_LIB_PATH.exists() and TORCH_LIB_PATH.stat().st_mtime >= newest
+            and TORCH_STAMP_PATH.exists() and TORCH_STAMP_PATH.read_text().strip() == torch_stamp())
 
 
 def _run(cmd, verbose):
@@ -86,13 +90,19 @@ def _run(cmd, verbose):
     return res.stdout + res.stderr
 
 
-def build_torch_lib(force: bool = False, verbose: bool = False) -> Path:
+def build_torch_lib(force: bool = False, verbose: bool = False) -> Optional[Path]:
     """Compile the operators implemented in C++ against the installed torch; they call libspio_b200, which lies
-    beside them."""
+    beside them.  Without a torch that has CUDA libraries there is nothing to link them with: the C-ABI library is
+    then all that is built, and the operators' calls say that theirs is missing."""
+    try:
+        import torch
+    except ImportError:
+        torch = None
+    if torch is None or torch.version.cuda is None:
+        print("torch with CUDA is not installed: the PyTorch operators in C++ are not built", file=sys.stderr)
+        return None
     if not force and torch_lib_is_current():
         return TORCH_LIB_PATH
-    import torch
-
     root = Path(torch.__file__).resolve().parent
     cuda = Path(find_nvcc()).resolve().parent.parent
     _run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-w",
@@ -101,6 +111,7 @@ def build_torch_lib(force: bool = False, verbose: bool = False) -> Path:
           f"-I{cuda / 'include'}", str(TORCH_SOURCE), "-o", str(TORCH_LIB_PATH),
           f"-L{LIB_DIR}", "-lspio_b200", "-Wl,-rpath,$ORIGIN",
           f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch"], verbose)
+    TORCH_STAMP_PATH.write_text(torch_stamp() + "\n")
     return TORCH_LIB_PATH
 
 

@@ -37,8 +37,7 @@ _fragment.define("checkpoint8_unpack(Tensor codes, Tensor exponents, ScalarType 
 # conv2d_gw8_checkpoint8 for plain eager calls, with the tile configurations of its three kernels
 _fragment.define("conv2d_gw8_checkpoint8_planned(Tensor inputs, Tensor weight, Tensor? bias, int padding_y, "
                  "int padding_x, int[] tunes) -> Tensor")
-if _clib.TORCH_LIB_PATH.exists():
-    _clib.load_torch_ops()
+_clib.load_torch_ops_if_usable()
 
 checkpoint8_pack_op = torch.ops.spio.checkpoint8_pack
 checkpoint8_unpack_op = torch.ops.spio.checkpoint8_unpack

@@ -32,8 +32,7 @@ _fragment.define("groupnorm_2d_forward(Tensor x, Tensor? weight, Tensor? bias, i
 _fragment.define("groupnorm_2d_backward(Tensor grad_output, Tensor? x, Tensor? codes, Tensor? exponents, Tensor stats, "
                  "Tensor? weight, Tensor? bias, int num_groups, str activation, bool needs_input_grad, "
                  "bool needs_weight_grad, bool needs_bias_grad) -> (Tensor, Tensor, Tensor)")
-if _clib.TORCH_LIB_PATH.exists():
-    _clib.load_torch_ops()
+_clib.load_torch_ops_if_usable()
 
 groupnorm_2d_op = torch.ops.spio.groupnorm_2d_forward
 groupnorm_2d_backward_op = torch.ops.spio.groupnorm_2d_backward

@@ -69,7 +69,9 @@ def _transform(model: torch.nn.Module, group_norm: bool = False,
         module = traced.get_submodule(target)
         cls = _matching_class(module)
         if cls is not None:
-            new = cls.from_torch_module(module, checkpoint8=checkpoint8)
+            # (a class that a user has added to the list need not know the option)
+            options = {"checkpoint8": True} if checkpoint8 and hasattr(cls, "checkpoint8") else {}
+            new = cls.from_torch_module(module, **options)
         elif group_norm and GroupNorm2d.match(module):
             new = _replace_group_norm(traced, nodes, checkpoint8)
         else:

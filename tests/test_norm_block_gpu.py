@@ -205,3 +205,25 @@ def test_transform_keeps_activations_that_it_must_not_take_in():
     for name in ("norm", "shared"):                 # the graph itself, with torch's layer back in place
         setattr(fast, name, getattr(net, name))
     assert all(torch.equal(p, q) for p, q in zip(fast(x, z, q), net(x, z, q)))
+
+
+@pytest.mark.parametrize("checkpoint8", [False, True])
+def test_transform_with_a_layer_class_of_the_user(monkeypatch, checkpoint8):
+    """A class in the list of layers needs no more than it always did: match and from_torch_module(module)."""
+    from spio_b200.transform import _transform
+
+    class Twice(nn.Module):
+        @staticmethod
+        def match(module):
+            return isinstance(module, nn.Identity)
+
+        @staticmethod
+        def from_torch_module(module):
+            return Twice()
+
+        def forward(self, x):
+            return 2 * x
+
+    monkeypatch.setattr(_transform, "spio_modules_classes", _transform.spio_modules_classes + [Twice])
+    fast = _transform.transform(nn.Sequential(nn.Identity(), nn.Conv2d(16, 16, 3, groups=2)), checkpoint8=checkpoint8)
+    assert isinstance(getattr(fast, "0"), Twice) and getattr(fast, "1").checkpoint8 == checkpoint8

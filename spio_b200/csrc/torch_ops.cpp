@@ -380,8 +380,20 @@ struct Conv {
   spio_gw8_tune fprop, dgrad, wgrad;
 };
 
-Conv conv_of(const Tensor& x, const Tensor& weight, const OptTensor& bias, int64_t pad_y, int64_t pad_x,
-             at::IntArrayRef tunes) {
+constexpr size_t kTunes = 3 * sizeof(spio_gw8_tune) / sizeof(int);
+
+Conv conv_of(at::IntArrayRef size, const Tensor& weight, int64_t pad_y, int64_t pad_x, at::IntArrayRef tunes) {
+  TORCH_CHECK_VALUE(tunes.size() == kTunes, "three tile configurations expected");
+  Conv c;
+  c.shape = {(int)size[0], (int)size[1], (int)size[2], (int)size[3], (int)weight.size(2), (int)weight.size(3),
+             (int)pad_y, (int)pad_x};
+  spio_gw8_tune* tune[3] = {&c.fprop, &c.dgrad, &c.wgrad};
+  for (size_t i = 0; i < kTunes; ++i) reinterpret_cast<int*>(tune[i / (kTunes / 3)])[i % (kTunes / 3)] = (int)tunes[i];
+  return c;
+}
+
+Conv checked_conv(const Tensor& x, const Tensor& weight, const OptTensor& bias, int64_t pad_y, int64_t pad_x,
+                  at::IntArrayRef tunes) {
   check_image(x, "conv2d_gw8_checkpoint8");
   TORCH_CHECK_VALUE(x.scalar_type() == at::kHalf && weight.scalar_type() == at::kHalf && weight.dim() == 4,
                     "conv2d_gw8 takes float16 data and weights");
@@ -390,15 +402,7 @@ Conv conv_of(const Tensor& x, const Tensor& weight, const OptTensor& bias, int64
   TORCH_CHECK_VALUE(!bias.has_value() || (bias->scalar_type() == at::kFloat && bias->dim() == 1 &&
                                           bias->size(0) == x.size(1) && bias->device() == x.device()),
                     "bias must be an fp32 vector of the channels on the data's device");
-  constexpr size_t kFields = sizeof(spio_gw8_tune) / sizeof(int);
-  TORCH_CHECK_VALUE(tunes.size() == 3 * kFields, "three tile configurations expected");
-  Conv c;
-  c.shape = {(int)x.size(0), (int)x.size(1), (int)x.size(2), (int)x.size(3), (int)weight.size(2), (int)weight.size(3),
-             (int)pad_y, (int)pad_x};
-  spio_gw8_tune* tune[3] = {&c.fprop, &c.dgrad, &c.wgrad};
-  for (size_t i = 0; i < 3; ++i)
-    for (size_t j = 0; j < kFields; ++j) reinterpret_cast<int*>(tune[i])[j] = (int)tunes[i * kFields + j];
-  return c;
+  return conv_of(x.sizes(), weight, pad_y, pad_x, tunes);
 }
 
 Tensor conv_forward(const Conv& c, const Tensor& x, const Tensor& weight, const OptTensor& bias_) {
@@ -412,19 +416,20 @@ Tensor conv_forward(const Conv& c, const Tensor& x, const Tensor& weight, const 
 
 Tensor conv2d_gw8_checkpoint8_planned(const Tensor& x, const Tensor& weight, const OptTensor& bias, int64_t pad_y,
                                       int64_t pad_x, at::IntArrayRef tunes) {
-  return conv_forward(conv_of(x, weight, bias, pad_y, pad_x, tunes), kernel_layout(x), weight, bias);
+  return conv_forward(checked_conv(x, weight, bias, pad_y, pad_x, tunes), kernel_layout(x), weight, bias);
 }
 
 struct ConvCheckpoint8 : torch::autograd::Function<ConvCheckpoint8> {
   static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x_, const Tensor& weight,
                         const OptTensor& bias, int64_t pad_y, int64_t pad_x, std::vector<int64_t> tunes) {
     at::AutoDispatchBelowADInplaceOrView below;
-    const Conv c = conv_of(x_, weight, bias, pad_y, pad_x, tunes);
+    const Conv c = checked_conv(x_, weight, bias, pad_y, pad_x, tunes);
     const Tensor x = kernel_layout(x_);
     const Tensor y = conv_forward(c, x, weight, bias);
-    auto [codes, exponents] = checkpoint8_pack(x);
+    Tensor codes, exponents;  // nothing but the weight's gradient reads the input's values again
+    if (weight.requires_grad()) std::tie(codes, exponents) = checkpoint8_pack(x);
     ctx->save_for_backward({codes, exponents, weight, tensor_of(bias)});
-    tunes.push_back(pad_y), tunes.push_back(pad_x);
+    for (const int64_t v : {pad_y, pad_x, x.size(0), x.size(1), x.size(2), x.size(3)}) tunes.push_back(v);
     ctx->saved_data["call"] = std::move(tunes);
     return y;
   }
@@ -438,16 +443,16 @@ struct ConvCheckpoint8 : torch::autograd::Function<ConvCheckpoint8> {
     const Tensor &codes = saved[0], &exponents = saved[1], &weight = saved[2];
     const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
     const bool want_b = saved[3].defined() && ctx->needs_input_grad(2);
-    const c10::cuda::CUDAGuard guard(codes.device());
-    // the sizes of the input are those of its codes; its values are read for the weight gradient alone
-    const Tensor x = want_w ? checkpoint8_unpack(codes, exponents, at::kHalf) : empty_image(codes.sizes(), codes, at::kHalf);
-    const std::vector<int64_t> call = ctx->saved_data["call"].toIntVector();  // tunes, padding
-    const Conv c = conv_of(x, weight, optional_of(saved[3]), call[call.size() - 2], call.back(),
-                           at::IntArrayRef(call).slice(0, call.size() - 2));
+    const c10::cuda::CUDAGuard guard(weight.device());
+    const std::vector<int64_t> call = ctx->saved_data["call"].toIntVector();  // tunes, padding, the input's size
+    const at::IntArrayRef tunes = at::IntArrayRef(call).slice(0, kTunes), size = at::IntArrayRef(call).slice(kTunes + 2, 4);
+    const Conv c = conv_of(size, weight, call[kTunes], call[kTunes + 1], tunes);
+    Tensor x;
+    if (want_w) x = checkpoint8_unpack(codes, exponents, at::kHalf);
     const Tensor dy = kernel_layout(grads[0]), w = kernel_layout(weight);
     Tensor dx, dw, db;
-    if (want_x) dx = empty_image(x.sizes(), x, at::kHalf);
-    if (want_w) dw = empty_image(weight.sizes(), weight, at::kHalf);
+    if (want_x) dx = empty_image(size, dy, at::kHalf);
+    if (want_w) dw = empty_image(weight.sizes(), dy, at::kHalf);
     // with an odd number of taps the weight-gradient kernel sums dy in a spare half of its last product
     const bool with_taps = want_b && want_w && (c.shape.r * c.shape.s) % 2 == 1;
     if (with_taps) db = empty_vector(c.shape.c, dy, at::kFloat);

@@ -96,11 +96,12 @@ def _conv2d_gw8_checkpoint8_fake(inputs, weight, bias=None, stride: int = 1, pad
 
 
 def _setup_context(ctx, inputs, output):
-    _x, weight, bias, _stride, padding_y, padding_x, *_ = inputs
+    x, weight, bias, _stride, padding_y, padding_x, *_ = inputs
     _y, codes, exponents = output
     ctx.mark_non_differentiable(codes, exponents)
-    ctx.save_for_backward(codes, exponents, weight, bias)
-    ctx.padding = (padding_y, padding_x)
+    kept = (codes, exponents) if ctx.needs_input_grad[1] else (None, None)   # for the weight gradient alone
+    ctx.save_for_backward(*kept, weight, bias)
+    ctx.padding, ctx.size = (padding_y, padding_x), x.shape
 
 
 def _backward(ctx, grad_output, _grad_codes, _grad_exponents):
@@ -108,7 +109,8 @@ def _backward(ctx, grad_output, _grad_codes, _grad_exponents):
     need = ctx.needs_input_grad
     want = (need[0], need[1], need[2] and bias is not None)
     # only the weight gradient reads the input's values; the others take its shape and type from `x`
-    x = _unpack(codes, exponents, torch.float16) if want[1] else torch.empty_like(codes, dtype=torch.float16)
+    x = (_unpack(codes, exponents, torch.float16) if want[1]
+         else torch.empty(ctx.size, dtype=torch.float16, device=weight.device, memory_format=torch.channels_last))
     grads = conv2d_gw8_backward_op(x, weight, bias, grad_output, *ctx.padding, *want)
     return tuple(g if w else None for g, w in zip(grads, want)) + (None,) * 5
 
@@ -164,16 +166,16 @@ def conv2d_gw8_checkpoint8(inputs: torch.Tensor, weight: torch.Tensor, bias: Opt
                            stride: int = 1, padding_y: int = 0, padding_x: int = 0, dilation: int = 1,
                            groups: int = 1) -> torch.Tensor:
     """:func:`conv2d_gw8` that keeps the 8-bit form of ``inputs`` for the backward pass (1.125 bytes a value
-    instead of 2).  Output, input gradient and bias gradient are those of :func:`conv2d_gw8`; the weight gradient
+    instead of 2; nothing where the weight requires no gradient).  Output, input gradient and bias gradient are those of :func:`conv2d_gw8`; the weight gradient
     is taken at the restored input."""
     if has_torch_function((inputs, weight, bias)):      # a torch.fx proxy, a tensor subclass
         return handle_torch_function(conv2d_gw8_checkpoint8, (inputs, weight, bias), inputs, weight, bias, stride=stride,
                                      padding_y=padding_y, padding_x=padding_x, dilation=dilation, groups=groups)
     _clib.load_torch_ops()
-    if torch.is_grad_enabled() and weight.requires_grad:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (inputs, weight, bias)):
         tunes = _eager_tunes(inputs, weight, bias, stride, padding_y, padding_x, dilation, groups)
         if tunes is not None:
             return _conv_planned(inputs, weight, bias, padding_y, padding_x, tunes)
         return conv2d_gw8_checkpoint8_op(inputs, weight, bias, stride, padding_y, padding_x, dilation, groups)[0]
-    # nothing will read the input again
+    # nothing is kept
     return conv2d_gw8(inputs, weight, bias, stride, padding_y, padding_x, dilation, groups)

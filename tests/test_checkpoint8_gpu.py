@@ -206,3 +206,57 @@ def test_memory_kept_for_the_backward_pass():
         kept.append(torch.cuda.memory_allocated() - before - 2 * size)
         del y
     assert kept[0] >= 2 * size and kept[1] <= 1.125 * size + (1 << 20), kept
+
+
+def test_a_frozen_weight_keeps_no_input():
+    """Without a weight gradient nothing reads the input again, and neither it nor its codes are kept."""
+    sh = O.Shape(8, 64, 56, 56, 3, 3, 1, 1)
+    w, b = torch.randn(64, 8, 3, 3, device="cuda").half(), torch.randn(64, device="cuda")
+    conv2d_gw8_checkpoint8(torch.zeros(8, 64, 56, 56, device="cuda").half(), w, b, padding_y=1, padding_x=1, groups=8)
+    for trained_bias in (False, True):
+        bias = b.clone().requires_grad_(trained_bias)
+        gc.collect()
+        torch.cuda.synchronize()
+        leaf = torch.randn(sh.n, sh.c, sh.h, sh.w, device="cuda").half().contiguous(memory_format=CL).requires_grad_(True)
+        dy = torch.randn_like(leaf)
+        before = torch.cuda.memory_allocated()
+        x = leaf * 2
+        y = conv2d_gw8_checkpoint8(x, w, bias, padding_y=1, padding_x=1, groups=8)
+        size = y.numel()
+        del x
+        torch.cuda.synchronize()
+        assert torch.cuda.memory_allocated() - before - 2 * size <= 1 << 20
+        torch.cuda.reset_peak_memory_stats()
+        held = torch.cuda.memory_allocated()
+        got = torch.autograd.grad(y, [leaf] + [bias] * trained_bias, dy)
+        torch.cuda.synchronize()
+        assert torch.cuda.max_memory_allocated() - held <= 2 * (2 * size) + (1 << 20)      # the two gradients of the input
+        del y
+        want = torch.autograd.grad(conv2d_gw8(leaf * 2, w, bias, 1, 1, 1, 1, 8), [leaf] + [bias] * trained_bias, dy)
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+        del got, want, leaf, dy
+
+
+def test_a_frozen_weight_under_autocast():
+    """The Python operator, which packs but keeps nothing."""
+    sh = O.Shape(8, 64, 56, 56, 3, 3, 1, 1)
+    w = torch.randn(64, 8, 3, 3, device="cuda")
+
+    def step(conv, x):
+        with torch.autocast("cuda", dtype=torch.float16):
+            return conv(x, w, None, 1, 1, 1, 1, 8)
+
+    kept = []
+    for conv in (conv2d_gw8, conv2d_gw8_checkpoint8):
+        x = torch.randn(sh.n, sh.c, sh.h, sh.w, device="cuda").contiguous(memory_format=CL).requires_grad_(True)
+        step(conv, x)
+        gc.collect()
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        y = step(conv, x)
+        torch.cuda.synchronize()
+        kept.append(torch.cuda.memory_allocated() - before - 4 * y.numel())
+        dy = torch.randn_like(y)
+        assert torch.equal(torch.autograd.grad(y, x, dy)[0], torch.autograd.grad(step(conv2d_gw8, x), x, dy)[0])
+        del y, dy
+    assert kept[1] <= 1 << 20 < kept[0], kept

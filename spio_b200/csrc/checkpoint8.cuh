@@ -11,8 +11,8 @@
 //
 // Why powers of two and blocks of 8: scaling is exact, so codes are a function of the input alone,
 // whatever arithmetic computes them, and a block is one thread's piece: no shuffles, and any split of
-// the channels over threads and CTAs sees whole blocks.  1.125 bytes a value; the largest magnitude
-// of 8 values is 1.42 standard deviations for normal data, so the step is 1.4 / 91 of one on average.
+// the channels over threads and CTAs sees whole blocks.  1.125 bytes a value; for normal data
+// the largest magnitude of 8 values is 1.78 standard deviations on average, and the step 1 / 49 of one.
 #pragma once
 
 #include <cuda_bf16.h>

@@ -235,21 +235,23 @@ void set_ring(Plan* p, int type, int bytes, bool backward) {
 // device, wide slabs whole DRAM sectors, few CTAs little bookkeeping, two launches any number of CTAs for one
 // image.  The costs are estimates in cycles with constants fitted to 14000 measured launches of 300 sizes (all types,
 // activations and directions; 0.2 to 64 million values): the choice takes 3 % longer than the best of each size on
-// average, 42 % at worst (28 us instead of 19).
+// average, 15 % or more at one size in 13 and 42 % at worst (28 us instead of 19).
 struct Work {
-  double values, piece, piece_bytes, read, written;  // piece: instructions a warp spends on it in both passes
+  double piece, piece_bytes;  // instructions a warp spends on a piece in both passes, bytes of it
+  double read, written;       // bytes, each once
 };
 
 Work work_of(const spio_groupnorm_2d_desc* d, bool backward, bool coded) {
-  static const double smooth[kActs] = {0., .2, 1., 1.8};
+  static const double smooth[kActs] = {0., .2, 1., 1.8};  // instructions of an activation, in those of SiLU
   const double act = smooth[d->activation] * (d->type == 2 ? 2.2 : 1.);  // (fp32: exact functions)
   const double size = d->type == 2 ? 4 : 2;
+  const double values = (double)d->n * d->pixels * d->c;
   Work w;
-  w.values = (double)d->n * d->pixels * d->c;
   w.piece_bytes = 8 * size;
+  // copies, conversions, sums and stores; the activation (twice backward); the codes; for fp32 the second word of a piece
   w.piece = (backward ? 110 + 85 * act + (coded ? 20 : 0) : 72 + 28 * act + (coded ? 25 : 0)) + (d->type == 2 ? 15 : 0);
-  w.read = w.values * (backward ? size + (coded ? 1.125 : size) : size);
-  w.written = w.values * (size + (coded && !backward ? 1.125 : 0));
+  w.read = values * (backward ? size + (coded ? 1.125 : size) : size);
+  w.written = values * (size + (coded && !backward ? 1.125 : 0));
   return w;
 }
 
@@ -262,15 +264,19 @@ double cost_of_one_launch(const Plan& p, const Work& w, const Device& dev, bool 
   const int on_sm = std::max(1, std::min((backward ? 512 : 768) / p.threads, 228 * 1024 / (p.smem + 1024)));
   const double of_sm = std::ceil(ctas / dev.sms), rounds = std::ceil(of_sm / on_sm);
   const double warps = std::min(of_sm, (double)on_sm) * p.threads / 32;
+  // a warp's bookkeeping and reductions, more of them where groups cut pieces, and its pieces; an SM issues up to 3.9 a
+  // cycle, a warp .358
   const double instructions = of_sm * p.threads / 32 * ((backward ? 969 : 645) + (g.fold ? 0 : 195) + pieces * w.piece);
   const double compute = instructions / std::min(3.9, .358 * warps);
   const double row = g.sp * w.piece_bytes;
-  const double again = std::max(0., 1. - (double)p.slots / pieces) * w.read * (backward ? .845 : 2.54);  // from L2
+  // what the ring no longer holds is read again, from L2 or DRAM, in bytes of the first reading that take as long
+  const double again = std::max(0., 1. - (double)p.slots / pieces) * w.read * (backward ? .845 : 2.54);
   const double filled = std::min(1., 2.19 * ctas * p.threads / (dev.sms * 256.));  // few threads have little on its way
-  const double memory =
+  const double memory =  // (pixels' rows below 64 bytes leave sectors half used)
       (w.read + w.written + again) / kBytesPerCycle / (row >= 64 ? 1. : row >= 32 ? .6 : .36) / filled;
-  const double sync = g.cluster > 1 ? 380 + 587 * g.log_cluster : 0;
-  // (the CTAs of an SM start together, and load and compute in turn more than at a time)
+  const double sync = g.cluster > 1 ? 380 + 587 * g.log_cluster : 0;  // starting a cluster, its barriers and loads
+  // the CTAs of an SM start together, and load and compute in turn more than at a time: weights of the longer and the
+  // shorter; then what each round of CTAs waits for in a row, and launches (backward: the sum of the parts too)
   return .82 * std::max(compute, memory) + 1.45 * std::min(compute, memory) +
          rounds * ((backward ? 1620 : 1270) + sync) + (backward ? 6890 : 3490);
 }
@@ -280,11 +286,13 @@ double cost_of_two_launches(const Plan& p, const Work& w, const Device& dev, boo
   if (g.parts == 1) return std::numeric_limits<double>::infinity();  // the same CTAs do it in one launch
   const double of_sm = std::ceil((double)g.images * g.slabs * g.parts / dev.sms);
   const int pieces = cdiv(cdiv(g.pixels, g.parts), p.threads / g.sp);
-  const double compute = of_sm * p.threads / 32 * (458 + pieces * (w.piece + 10)) / 2.28;
+  const double compute = of_sm * p.threads / 32 * (458 + pieces * (w.piece + 10)) / 2.28;  // as above; 2.28 a cycle
   // pixels' segments that begin and end inside a cache line cost where L2 does not hold them until the rest is wanted
   const double row = g.sp * w.piece_bytes, beyond = std::min(1., std::max(0., (w.read + w.written - 5e7) / 1e8));
   const double torn = g.slabs > 1 && (g.sp * (int)w.piece_bytes) % 128 != 0 ? 14.5 / row * beyond : 0.;
+  // (a quarter of the second reading is paid for, the rest is in L2)
   const double memory = (1.25 * w.read + w.written) * (1. + torn) / kBytesPerCycle;
+  // rounds of loads in which a CTA of the second launch merges the parts
   const double merges = cdiv(g.slab_groups, 8 * (backward ? 4 : 2)) * cdiv(g.parts / g.cluster, 256);
   return .9 * std::max(compute, memory) + .73 * std::min(compute, memory) + 1020 * merges + (backward ? 14000 : 10100);
 }

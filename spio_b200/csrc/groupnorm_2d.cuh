@@ -41,9 +41,10 @@ __device__ __forceinline__ float reciprocal_approx(float x) {
   return r;
 }
 // EXACT: for fp32 data, CUDA's own functions.  Otherwise results are rounded to 11 bits or fewer, and the
-// hardware's exponential and reciprocal (relative errors of some 2^-22) are far below that; erfc is
-// Abramowitz and Stegun's 7.1.26 (absolute error 1.5e-7, with a factor exp(-x^2) that keeps the tail's
-// relative error below the rounding of 16-bit types).
+// hardware's exponential and reciprocal (relative errors of some 2^-22) are far below that.  The normal distribution
+// function is then Abramowitz and Stegun's 7.1.26, off by 7e-8 at most, and GELU by 2.2e-7: for negative z within half a
+// step of fp16 down to -3.6 and of bf16 down to -5.3.  Further out, where GELU is 6e-4 and less, its relative error
+// grows: 0.05 % at -4, 0.4 % at -6 (half a step of bf16 is 0.2 to 0.4 %), 1 % at -8, 3 % at -12.
 template <int ACT, bool EXACT>
 struct Activation {
   static __device__ __forceinline__ float exact_sigmoid(float z) { return 1.f / (1.f + expf(-z)); }
@@ -1021,15 +1022,17 @@ groupnorm_2d_bwd_apply_kernel(T* __restrict__ dx, const float2* __restrict__ par
 // memory, so one launch does both passes and the second one finds its data close by: it goes through the pieces
 // backwards, those that are still in the ring first (all of them, where a part fits), the others again from L2.
 //
-// Measured at 256 x 64 x 56 x 56 fp16 with SiLU and 8 groups: 49.6 us forward (4140 GB/s counting x and y once, 64 % of
-// what a copy reaches), 85.4 us backward with the sum of the parts (3610 GB/s, 55 %); 28.4 and 41.5 us at
-// 128 x 192 x 28 x 28 with 8-bit codes.  Nothing is used up: forward 51 % of the issue slots and 51 % of the special
-// functions (two a value), backward 49 % and 59 % (four a value).  The CTAs of an SM begin together, so that they load and
-// compute in turn more than at a time.  What did not help: a CTA that goes on to the next image and requests it
-// during its second pass (the bookkeeping of an image came back as waiting), five CTAs of 96 registers instead of four of
-// 128 (88.6 us backward), smaller parts (the second pass of the backward kernel finds 120 of 206 MB no longer in L2; with
-// parts of a quarter of that size it takes 88.3 us, because they pay the reductions more often), one reciprocal for
-// two values, keeping the first pass's gradients in shared memory.
+// Measured at 256 x 64 x 56 x 56 fp16 with SiLU and 8 groups: 49.9 us forward (4120 GB/s counting x and y once, 63 % of
+// what a copy reaches), 87.0 us backward with the sum of the parts (3550 GB/s, 54 %); 29.6 and 42.4 us at
+// 128 x 192 x 28 x 28 with 8-bit codes.  Nothing is used up: forward 53 % of the issue slots and 53 % of the special
+// functions (two a value), backward 50 % and 59 % (four a value).  What bounds them is this structure: a thread asks for
+// its own 16 bytes at a time and waits for them, and the CTAs of an SM begin together, so that they load and compute in
+// turn more than at a time.  It is not the activation: 53 and 85 us without one.  What did not help: a CTA
+// that goes on to the next image and requests it during its second pass (the bookkeeping of an image came back as
+// waiting, in every warp), five CTAs of 96 registers instead of four of 128 (88.6 us backward instead of 87 then),
+// smaller parts (the second pass of the backward kernel finds 130 of 206 MB no longer in L2; parts of a quarter of that
+// size took 88.3 us, because they pay the reductions more often), one reciprocal for two values, keeping the first
+// pass's gradients in shared memory.  Not tried: a producer warp that fetches whole rows by bulk copies for the others.
 
 template <class T, int ACT, bool CODES>
 __global__ void __launch_bounds__(kGnThreads, 768 / kGnThreads)

@@ -5,8 +5,9 @@ A block of 8 consecutive channels of a pixel -- one channel group of the gw8 con
 codes and one exponent byte and stands for ``code * 2**(exponent - 127)``: 1.125 bytes a value.  The scale is
 the smallest power of two (``2**-126`` at least) for which the block's largest magnitude rounds to at most 127,
 so a restored value is off by at most half a step, 1/127 of the block's largest magnitude.  (Where rounding up
-would leave the range of the type, codes stop at 63 and the error is up to 1/64 of that magnitude.)  A block with an infinity or a NaN
-is restored as NaN, so that a gradient scaler still finds it.
+would leave the range of the type, codes stop at 63 and the error is up to 1/64 of that magnitude.  Where the scale
+is at its floor the error is up to ``2**-127``, which may be all of a value.)  A block with an infinity or a NaN is
+restored as NaN, so that a gradient scaler still finds it.
 
 The reference keeps the convolution's input as it is (spio/functional/conv2d_gw8_function.py:150-171); this
 form has no counterpart there.  The device work is done by libspio_b200 on torch's current stream; CPU tensors

@@ -1,9 +1,10 @@
-"""When an operator may be called without torch's dispatcher.
+"""When a call of a Python operator may take its C++ form instead.
 
 A Python operator costs 20 to 50 us of host time in eager mode (about 200 us with its backward pass), more than
-the kernels of a small tensor.  Plain eager calls therefore go through ``torch.autograd.Function``; everything that has to see an operator -- fake tensors,
-tensor subclasses, tracing and compilation, functorch transforms, forward-mode derivatives, dispatch modes such as
-profilers' counters -- still finds the custom operator.
+the kernels of a small tensor.  A plain eager call of the convolution with the 8-bit checkpoint therefore takes an
+operator in C++ (csrc/torch_ops.cpp); whatever has to see the public operator -- fake tensors, tensor subclasses,
+tracing and compilation, functorch transforms, forward-mode derivatives, dispatch modes such as profilers'
+counters -- still finds that.
 """
 
 from __future__ import annotations
